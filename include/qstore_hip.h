@@ -415,6 +415,75 @@ int qs_quant_rows_lowbit(const float* W, int64_t ldw, int64_t N, int64_t K, int 
                          uint8_t* packed, int64_t row_bytes, float* scales, uint8_t* codes,
                          void* stream);
 
+/* ---- attention over a paged 4-bit KV cache ------------------------------------------------
+ * No counterpart in the reference's QStore path: what lies between a layer's q/k/v linears and its
+ * output projection, over a cache in the weights' spirit (codes with a scale and a lowest value). */
+
+/* Paging metadata of a step from request lengths: request b has past[b] tokens in the cache and
+ * fresh[b] new ones (negative: 0), P = page_size (a power of two).  It owns ceil(past/P) table
+ * columns and takes ceil((past + fresh)/P) - ceil(past/P) pages, in request order, from the ring of
+ * free pages: state = {head, tail, missing} int64, free pages are ring[head .. tail-1 mod ring_size].
+ * Written: tables[b*ld_table + column] of new columns (-1 where no page was left), and for row t of
+ * T: slots (page*P + offset, -1 for padding or without a page), positions, requests (-1: padding);
+ * starts[B+1], context[B] = past + fresh; state_out (not state): the head moved, missing = pages not
+ * given.  Rows beyond T and columns beyond width take no page. */
+int qs_plan_step(const int32_t* ring, int64_t ring_size, const int64_t* state, int64_t* state_out,
+                 int32_t* tables, int64_t ld_table, int64_t width, const int32_t* past,
+                 const int32_t* fresh, int64_t B, int64_t page_size, int64_t T, int64_t* slots,
+                 int32_t* positions, int32_t* requests, int32_t* starts, int32_t* context,
+                 void* stream);
+
+/* Pages of requests with done[b] != 0, which hold lens[b] tokens, back to the ring's tail, in request
+ * and column order; entries below 0 are passed over.  state_out = {head, new tail, 0}. */
+int qs_release_pages(int32_t* ring, int64_t ring_size, const int64_t* state, int64_t* state_out,
+                     const int32_t* tables, int64_t ld_table, int64_t width, const int32_t* lens,
+                     const uint8_t* done, int64_t B, int64_t page_size, void* stream);
+
+/* Rotary positions of x [T, H, D] (F32/BF16/F16; strides ld*_t, ld*_h in elements, heads
+ * contiguous): the first rot values of a head turn by positions[t] * freq[i] (fp64 angles, cos and
+ * sin times magnitude rounded to fp32), pairs (i, i + rot/2) or with interleaved (2i, 2i+1); inverse
+ * turns back.  y may be x. */
+int qs_rotary(const void* x, int dtype, int64_t ldx_t, int64_t ldx_h, const int32_t* positions,
+              const double* freq, int rot, int interleaved, int inverse, double magnitude, void* y,
+              int64_t ldy_t, int64_t ldy_h, int64_t T, int H, int D, void* stream);
+
+/* Bytes of one (page, head) block of the cache; 0 for an unsupported shape (head_dim 64, 128, 256;
+ * page_size 16..256, a power of two).  A layer is [pages][Hkv][block bytes], 16-byte aligned. */
+size_t qs_kv4_block_bytes(int64_t head_dim, int64_t page_size);
+
+/* Codes k and v [T, Hkv, D] into slots[t] = page * page_size + offset (others are passed over), in
+ * groups of 64 values: lo = fp16(min), s = fp16((max - min)/15), code = clamp(rint((x - lo)/s), 0, 15)
+ * (0 where s is 0), a code standing for code * s + lo; NaN counts as 0, values are held to +-60000.
+ * With rot > 0 (a multiple of 8) keys are turned by positions[t] first as by qs_rotary and rounded to
+ * their type, and so are the queries q [T, Hq, D] (Hq may be 0) into q_out (contiguous). */
+int qs_kv4_append(const void* k, int64_t ldk_t, int64_t ldk_h, const void* v, int64_t ldv_t,
+                  int64_t ldv_h, int dtype, const int64_t* slots, uint8_t* cache, int64_t pages,
+                  int64_t page_size, int Hkv, int D, int64_t T, const void* q, int64_t ldq_t,
+                  int64_t ldq_h, int Hq, void* q_out, const int32_t* positions, const double* freq,
+                  int rot, int interleaved, double magnitude, void* stream);
+
+/* What n slots hold, [n, Hkv, D] each (k_out or v_out may be null); zeros for other slots. */
+int qs_kv4_read(const uint8_t* cache, int64_t pages, int64_t page_size, int Hkv, int D,
+                const int64_t* slots, int64_t n, void* k_out, void* v_out, int out_dtype,
+                void* stream);
+
+/* Workspace bytes of qs_kv4_attend for these sizes (0: none). */
+size_t qs_kv4_attend_workspace_bytes(int64_t T, int64_t B, int Hkv, int Hq, int D, int64_t page_size,
+                                     int64_t max_query, int64_t max_context, int64_t window);
+
+/* Causal attention of q [T, Hq, D] over the cache: request b's queries are rows starts[b] ..
+ * starts[b+1]-1 (starts[0] = 0), the last of its context[b] tokens, whose pages are tables[b*ld_table
+ * + column].  A query sees the tokens up to its own, with window > 0 the last `window` of them;
+ * tokens of a column past width, or whose entry is not in [0, pages), are not seen; a query that sees
+ * nothing, or a row after the last request's, gives zeros.  max_query / max_context bound the
+ * requests (0 or larger than the truth is fine; they only choose the split).  out [T, Hq, D]
+ * contiguous.  q heads are 16-byte aligned.  Calls that overlap need workspaces of their own. */
+int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ldq_h, const uint8_t* cache,
+                  int64_t pages, int64_t page_size, int Hkv, int Hq, int D, const int32_t* tables,
+                  int64_t ld_table, int64_t width, const int32_t* starts, const int32_t* context,
+                  int64_t B, int64_t T, int64_t max_query, int64_t max_context, float scale,
+                  int64_t window, void* out, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- pinned-host -> HBM page streaming -------------------------------------------------
  * Replaces the CUDA prefetch ring _RingSlot / _RingPrefetch (src/mrun/engine/kernels/
  * qstore.py:459-660: pinned staging, side-stream H2D, event + record_stream ordering) at

@@ -86,6 +86,14 @@ SIGNATURES: dict[str, tuple] = {
     "qs_lowbit_workspace_bytes": (ctypes.c_size_t, [_I, _L, _L, _L, _I]),
     "qs_lowbit_many_plan": (_I, [_I, _L, _L, _L, _I, _P]),
     "qs_lowbit_gemv": (_I, [_P, _I, _L, _P, _L, _P, _I, _P, _I, ctypes.c_float, _I, _I, _P, _L, _L, _L, _L, _P, ctypes.c_size_t, _P]),
+    "qs_plan_step": (_I, [_P, _L, _P, _P, _P, _L, _L, _P, _P, _L, _L, _L, _P, _P, _P, _P, _P, _P]),
+    "qs_release_pages": (_I, [_P, _L, _P, _P, _P, _L, _L, _P, _P, _L, _L, _P]),
+    "qs_rotary": (_I, [_P, _I, _L, _L, _P, _P, _I, _I, _I, ctypes.c_double, _P, _L, _L, _L, _I, _I, _P]),
+    "qs_kv4_block_bytes": (ctypes.c_size_t, [_L, _L]),
+    "qs_kv4_append": (_I, [_P, _L, _L, _P, _L, _L, _I, _P, _P, _L, _L, _I, _I, _L, _P, _L, _L, _I, _P, _P, _P, _I, _I, ctypes.c_double, _P]),
+    "qs_kv4_read": (_I, [_P, _L, _L, _I, _I, _P, _L, _P, _P, _I, _P]),
+    "qs_kv4_attend_workspace_bytes": (ctypes.c_size_t, [_L, _L, _I, _I, _I, _L, _L, _L, _L]),
+    "qs_kv4_attend": (_I, [_P, _I, _L, _L, _P, _L, _L, _I, _I, _I, _P, _L, _L, _P, _P, _L, _L, _L, _L, ctypes.c_float, _L, _P, _P, ctypes.c_size_t, _P]),
     "qs_pager_create": (_I, [_P, ctypes.c_size_t, _I, ctypes.c_size_t, ctypes.POINTER(_P)]),
     "qs_pager_destroy": (_I, [_P]),
     "qs_pager_slot_ptr": (_P, [_P, _I]),
