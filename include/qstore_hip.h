@@ -467,7 +467,9 @@ int qs_kv4_read(const uint8_t* cache, int64_t pages, int64_t page_size, int Hkv,
                 const int64_t* slots, int64_t n, void* k_out, void* v_out, int out_dtype,
                 void* stream);
 
-/* Workspace bytes of qs_kv4_attend for these sizes (0: none). */
+/* Workspace bytes of qs_kv4_attend for these sizes (0: none).  The workspace's first 32 KiB are zero
+ * before its first use, and every call leaves them zero: calls that follow one another on a stream
+ * can share one of the largest size, calls that overlap need workspaces of their own. */
 size_t qs_kv4_attend_workspace_bytes(int64_t T, int64_t B, int Hkv, int Hq, int D, int64_t page_size,
                                      int64_t max_query, int64_t max_context, int64_t window);
 
@@ -476,8 +478,8 @@ size_t qs_kv4_attend_workspace_bytes(int64_t T, int64_t B, int Hkv, int Hq, int 
  * + column].  A query sees the tokens up to its own, with window > 0 the last `window` of them;
  * tokens of a column past width, or whose entry is not in [0, pages), are not seen; a query that sees
  * nothing, or a row after the last request's, gives zeros.  max_query / max_context bound the
- * requests (0 or larger than the truth is fine; they only choose the split).  out [T, Hq, D]
- * contiguous.  q heads are 16-byte aligned.  Calls that overlap need workspaces of their own. */
+ * requests (0 or larger than the truth is fine; they only choose the split).  starts does not
+ * decrease.  out [T, Hq, D] contiguous.  q heads are 16-byte aligned. */
 int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ldq_h, const uint8_t* cache,
                   int64_t pages, int64_t page_size, int Hkv, int Hq, int D, const int32_t* tables,
                   int64_t ld_table, int64_t width, const int32_t* starts, const int32_t* context,

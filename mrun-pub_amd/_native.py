@@ -185,6 +185,26 @@ def inference(fn):
     return run
 
 
+_kept: dict[tuple[int, int], torch.Tensor] = {}
+SYNC_BYTES = 32768  # of a workspace's start, in which kernels count their blocks
+
+
+def kept_workspace(device: torch.device, stream: int, need: int) -> torch.Tensor:
+    """A workspace whose first ``SYNC_BYTES`` are zero, for kernels that leave them zero: one a
+    stream, whose calls follow one another.  A call that is captured into a graph, which may run
+    beside them, gets one of its own, cleared in the graph."""
+    if torch.cuda.is_current_stream_capturing():
+        fresh = torch.empty(need, dtype=torch.uint8, device=device)
+        fresh[:SYNC_BYTES].zero_()
+        return fresh
+    have = _kept.get((device.index, stream))
+    if have is None or have.numel() < need:
+        have = torch.empty(need, dtype=torch.uint8, device=device)
+        have[:SYNC_BYTES].zero_()
+        _kept[device.index, stream] = have
+    return have
+
+
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else int(t.data_ptr())
 

@@ -1,13 +1,15 @@
 // Attention over the paged 4-bit KV cache (gfx950).
 //
-//   k_kv4_attend : a wave takes 16 or 32 query rows of one KV head -- (new token, query head) pairs,
-//                  the heads that share the KV head next to each other -- and walks the request's
-//                  tokens 32 at a time; the waves of a block and the blocks of a split take every
-//                  NW-th step of their range and join their results.
-//   k_kv4_join   : joins the splits of a long context.
+//   k_attend_few  : up to 32 query rows of one KV head -- (new token, query head) pairs, the heads
+//                   that share the KV head next to each other -- a block.  Each wave takes all rows
+//                   over every NW-th step of 32 tokens, codes straight from memory into the matrix
+//                   instructions' operands; the waves' results join in LDS.
+//   k_attend_rows : 128 rows a block, 32 a wave; the block unpacks 64 tokens at a time into LDS,
+//                   where every wave reads them.
 //
 // o = sum_t p_t v_t / sum_t p_t with p_t = 2^(x_t - m), x the scores in units of log2 and m their
-// running maximum, one pass over the cache.
+// running maximum, one pass over the cache.  Blocks share the requests' tokens out among themselves
+// (pick_work); where several take parts of one tile's tokens, the last of them to finish joins them.
 #include "qs_kv4.h"
 #include "qs_values.h"
 
@@ -15,6 +17,8 @@ namespace qs {
 namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct AttendArgs {
   const void* q;
@@ -23,18 +27,43 @@ struct AttendArgs {
   const int* starts;
   const int* context;
   void* out;
-  float* part_o;
-  float2* part_ml;
+  float* part_o;    // [block][rows of a tile * D]
+  float2* part_ml;  // [block][rows of a tile]
+  int* done;        // [block]: parts finished of the tile whose first block it is; 0 between calls
   int64_t ldq_t, ldq_h, ld_table, T;
-  int pages, P, shift, width, Hkv, grp, B, window, splits;
+  int pages, P, shift, width, Hkv, grp, B, window;
+  int blocks, least;        // parts: blocks to fill, steps of a part at least; blocks 0: no parts
+  int rows_from, rows_upto;  // requests of other row counts are the other kernel's
   float scale_log2;
 };
 
 // ---- operand arithmetic ----------------------------------------------------------------
-// Eight values along the sum for the matrix instruction, of which 16-bit activations multiply
-// fp16: cache values are code * s + lo in fp16 (one rounding, 2^-12), queries are exact, since a
-// row of bf16 is first divided by a power of two that takes its largest value below 1 (8 bits fit
-// fp16's 11 down to 2^-17 of that), weights are 0..1.  fp32 activations multiply fp32.
+// A byte 0..15 read as an e4m3 number is byte * 2^-9 (subnormals below 8, one binade above), so one
+// conversion with scale 2^9 gives two codes as 16-bit floats.
+//
+// 16-bit activations multiply fp16: cache values are code * s + lo in fp16 (one rounding, 2^-11),
+// queries are exact, since a row of bf16 is first divided by a power of two that takes its largest
+// value below 1 (8 bits fit fp16's 11 down to 2^-17 of that), weights are fp16.
+//
+// fp32 activations are sums of three bf16 numbers (8 bits each, all of fp32's 24) and multiply the
+// codes, which bf16 holds exactly: q.k = s (q.code) + lo sum(q) a group, and for the output the
+// weights are p s, with p lo summed beside.  Three instructions of the 16-bit rate in place of the
+// fp32 instruction's sixteenfold time.
+constexpr uint32_t kNibbles = 0x0f0f0f0fu;
+
+template <class T>
+constexpr bool kCodes = sizeof(T) == 4;
+template <class T>
+constexpr int kParts = kCodes<T> ? 3 : 1;
+
+template <bool HI>
+__device__ __forceinline__ f16x2 f16_codes(uint32_t w) {
+  return __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 512.f, HI);
+}
+template <bool HI>
+__device__ __forceinline__ bf16x2 bf16_codes(uint32_t w) {
+  return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 512.f, HI);
+}
 
 template <class T>
 struct Ops {
@@ -42,262 +71,423 @@ struct Ops {
   static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ uint32_t pair(uint32_t w, int j) {  // codes j and j + 4 of w, as 1024 + c
-    return (w >> (4 * j) & 0x000f000fu) | 0x64006400u;
-  }
-  static __device__ __forceinline__ f16x2 value(uint32_t p, f16x2 s, f16x2 lo) {
-    const f16x2 off = {(_Float16)1024.f, (_Float16)1024.f};
-    return __builtin_elementwise_fma(__builtin_bit_cast(f16x2, p) - off, s, lo);
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
   // One dword of a token's key, and its (s, lo).
   static __device__ __forceinline__ Frag key(uint32_t w, uint32_t sl) {
     const f16x2 h = __builtin_bit_cast(f16x2, sl);
     const f16x2 s = {h[0], h[0]}, lo = {h[1], h[1]};
-    Frag f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const f16x2 v = value(pair(w, j), s, lo);
-      f[2 * j] = v[0];
-      f[2 * j + 1] = v[1];
-    }
-    return f;
+    const uint32_t a = w & kNibbles, b = w >> 4 & kNibbles;
+    const f16x2 v0 = __builtin_elementwise_fma(f16_codes<false>(a), s, lo);
+    const f16x2 v1 = __builtin_elementwise_fma(f16_codes<true>(a), s, lo);
+    const f16x2 v2 = __builtin_elementwise_fma(f16_codes<false>(b), s, lo);
+    const f16x2 v3 = __builtin_elementwise_fma(f16_codes<true>(b), s, lo);
+    return Frag{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
   }
-  // Values j (of four) of eight tokens: u holds the 16-bit words of token pairs, s and lo theirs.
-  static __device__ __forceinline__ Frag val(const uint32_t (&u)[4], const uint32_t (&s)[4], const uint32_t (&lo)[4], int j) {
+  // Values 4 m + J of eight tokens: u holds the bytes of token pairs, s and lo the pairs' own.
+  template <int J>
+  static __device__ __forceinline__ Frag val(const uint32_t (&u)[4], const uint32_t (&s)[4], const uint32_t (&lo)[4]) {
     Frag f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const f16x2 v = value(pair(u[i], j), __builtin_bit_cast(f16x2, s[i]), __builtin_bit_cast(f16x2, lo[i]));
+      const uint32_t w = (J & 1 ? u[i] >> 4 : u[i]) & kNibbles;
+      const f16x2 v = __builtin_elementwise_fma(f16_codes<(J >> 1) != 0>(w), __builtin_bit_cast(f16x2, s[i]),
+                                                __builtin_bit_cast(f16x2, lo[i]));
       f[2 * i] = v[0];
       f[2 * i + 1] = v[1];
     }
-    return f;
-  }
-  static __device__ __forceinline__ Frag weights(const float (&p)[8]) {
-    Frag f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = static_cast<_Float16>(p[i]);
     return f;
   }
 };
 
 template <>
 struct Ops<float> {
-  struct Frag {
-    float v[8];
-  };
-  static __device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[i], b.v[i], c, 0, 0, 0);
-    return c;
+  typedef bf16x8 Frag;
+  static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
-  static __device__ __forceinline__ Frag key(uint32_t w, uint32_t sl) {
-    const float s = f16_bits_to_f32((uint16_t)sl), lo = f16_bits_to_f32((uint16_t)(sl >> 16));
+  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ Frag key(uint32_t w, uint32_t) {
+    const uint32_t a = w & kNibbles, b = w >> 4 & kNibbles;
+    const bf16x2 v0 = bf16_codes<false>(a), v1 = bf16_codes<true>(a), v2 = bf16_codes<false>(b), v3 = bf16_codes<true>(b);
+    return Frag{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+  }
+  template <int J>
+  static __device__ __forceinline__ Frag val(const uint32_t (&u)[4], const uint32_t (&)[4], const uint32_t (&)[4]) {
     Frag f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = __builtin_fmaf((float)(w >> Kv4Layout::k_shift(e) & 15u), s, lo);
-    return f;
-  }
-  static __device__ __forceinline__ Frag val(const uint32_t (&u)[4], const uint32_t (&s)[4], const uint32_t (&lo)[4], int j) {
-    Frag f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int up = 16 * (i & 1);
-      f.v[i] = __builtin_fmaf((float)(u[i / 2] >> (up + 4 * j) & 15u), f16_bits_to_f32((uint16_t)(s[i / 2] >> up)),
-                              f16_bits_to_f32((uint16_t)(lo[i / 2] >> up)));
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = (J & 1 ? u[i] >> 4 : u[i]) & kNibbles;
+      const bf16x2 v = bf16_codes<(J >> 1) != 0>(w);
+      f[2 * i] = v[0];
+      f[2 * i + 1] = v[1];
     }
     return f;
   }
-  static __device__ __forceinline__ Frag weights(const float (&p)[8]) {
-    Frag f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f.v[i] = p[i];
-    return f;
-  }
 };
 
-// Maximum / sum over the four lanes of a query row (l, l ^ 16, l ^ 32, l ^ 48).
+// Eight fp32 values as operands: rounded to fp16, or as three bf16 parts.
+__device__ __forceinline__ void parts_of(const float (&v)[8], f16x8 (&p)[1]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[0][i] = static_cast<_Float16>(v[i]);
+}
+__device__ __forceinline__ void parts_of(const float (&v)[8], bf16x8 (&p)[3]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    p[0][i] = static_cast<__bf16>(v[i]);
+    const float r = v[i] - static_cast<float>(p[0][i]);
+    p[1][i] = static_cast<__bf16>(r);
+    p[2][i] = static_cast<__bf16>(r - static_cast<float>(p[1][i]));
+  }
+}
+
 __device__ __forceinline__ float max_of(float a, float b) { return a > b ? a : b; }
+// Maximum / sum over lanes l and l ^ 32, and over the four of l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float pair_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max_of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 __device__ __forceinline__ float quad_max(float v) {
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = max_of(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = pair_max(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return max_of(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float quad_sum(float v) {
-  auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = pair_sum(v);
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// ---- which rows a block has ---------------------------------------------------------------
-// Request b's tiles of R rows start at floor(starts[b] grp / R) + b, which leaves each request room
-// for its last, partial one and can be searched without sums over requests.  Tokens past the last
-// request are those of one more, with nothing to see.
-struct Tile {
-  int64_t q0;       // first token of the request
-  int b, n, row0;   // request, its new tokens, first row of the tile
+// A maximum is moved only by scores that pass it by 2^8: weights up to 256 lose nothing in fp16 or
+// fp32, and most steps then leave the sums alone.
+constexpr float kSlack = 8.f;
+
+// ---- which rows and tokens a block has -----------------------------------------------------
+struct Work {
+  int64_t q0;         // first token of the request
+  int b, n, row0;     // request, its new tokens, first row of the tile
+  int part, parts;    // which part of the tile's tokens, of how many
+  int64_t first;      // block of the tile's part 0
+  int hk;
   bool any;
 };
+
 __device__ __forceinline__ int64_t start_of(const AttendArgs& a, int b) {
   const int64_t s = b == 0 ? 0 : a.starts[b];
   return s < 0 ? 0 : s < a.T ? s : a.T;
 }
-__device__ __forceinline__ Tile find_tile(const AttendArgs& a, int64_t tile, int R) {
+// New tokens of request b; tokens past the last request are those of one more, with nothing to see.
+__device__ __forceinline__ int new_of(const AttendArgs& a, int b, int64_t q0) {
+  const int64_t q1 = b < a.B ? start_of(a, b + 1) : a.T;
+  return q1 > q0 ? (int)(q1 - q0) : 0;
+}
+__device__ __forceinline__ int context_of(const AttendArgs& a, int b) {
+  const int c = b < a.B ? a.context[b] : 0;
+  return c < 0 ? 0 : c < (1 << 30) ? c : 1 << 30;
+}
+__device__ __forceinline__ bool mine(const AttendArgs& a, int rows) { return rows >= a.rows_from && rows <= a.rows_upto; }
+
+// Without parts: request b's tiles of R rows start at floor(starts[b] grp / R) + b, which leaves each
+// request room for its last, partial one and can be searched without sums over requests.
+__device__ __forceinline__ Work pick_tile(const AttendArgs& a, int64_t y, int R) {
   const int lane = threadIdx.x & 63;
   int at = -1;
   for (int b0 = 0; b0 <= a.B; b0 += 64) {
     const int b = b0 + lane;
-    const bool before = b <= a.B && (int64_t)((uint64_t)(start_of(a, b) * a.grp) / (unsigned)R) + b <= tile;
+    const bool before = b <= a.B && (int64_t)((uint64_t)(start_of(a, b) * a.grp) / (unsigned)R) + b <= y;
     const int n = __popcll(__ballot(before));
     at += n;
     if (n < 64) break;
   }
-  Tile t;
+  Work t;
   t.b = at;
   t.q0 = start_of(a, at);
-  const int64_t q1 = at < a.B ? start_of(a, at + 1) : a.T;
-  t.n = q1 > t.q0 ? (int)(q1 - t.q0) : 0;
-  const int64_t row0 = (tile - ((int64_t)((uint64_t)(t.q0 * a.grp) / (unsigned)R) + at)) * R;
-  t.any = row0 >= 0 && row0 < (int64_t)t.n * a.grp;
-  t.row0 = (int)row0;
+  t.n = new_of(a, at, t.q0);
+  int64_t tile = y - ((int64_t)((uint64_t)(t.q0 * a.grp) / (unsigned)R) + at);
+  const int64_t tiles = ((int64_t)t.n * a.grp + R - 1) / R;
+  t.any = tile >= 0 && tile < tiles && mine(a, t.n * a.grp);
+  t.row0 = (int)((tiles - 1 - tile) * R);  // the last rows see most: they start first
+  t.part = 0;
+  t.parts = 1;
+  t.first = 0;
   return t;
 }
 
+// With parts: a tile whose tokens take W steps is cut into ceil(W / size) parts, size so that the
+// parts of all requests come to about a.blocks blocks.  Every block does the two sums over the
+// requests itself; each thread has B / threads of them.
+template <int R, int STEP, int THREADS>
+__device__ __forceinline__ Work pick_part(const AttendArgs& a, int64_t y, int64_t* s_sum, Work* s_work) {
+  const int each = a.B / THREADS + 1;  // of B + 1
+  const int b0 = threadIdx.x * each, b1 = b0 + each < a.B + 1 ? b0 + each : a.B + 1;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int NW = THREADS / 64;
+  int64_t q0;
+  int n = 0, tiles = 0, steps = 0;
+  auto look = [&](int b) {
+    q0 = start_of(a, b);
+    n = new_of(a, b, q0);
+    const int rows = n * a.grp;
+    tiles = mine(a, rows) ? (rows + R - 1) / R : 0;
+    const int ctx = context_of(a, b);
+    const int64_t reach = (int64_t)a.width << a.shift;
+    int64_t span = ctx < reach ? ctx : reach;
+    if (a.window > 0 && span > (int64_t)a.window + R) span = (int64_t)a.window + R;  // of one tile
+    steps = (int)((span + STEP - 1) / STEP);
+  };
+  auto block_sum = [&](int64_t v, int64_t& before) {
+    int64_t up = v;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t o = __shfl_up(up, off, 64);
+      if (lane >= off) up += o;
+    }
+    if (lane == 63) s_sum[wave] = up;
+    __syncthreads();
+    int64_t all = 0;
+    before = up - v;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < wave) before += s_sum[w];
+      all += s_sum[w];
+    }
+    __syncthreads();
+    return all;
+  };
+  int64_t sum = 0, before;
+  for (int b = b0; b < b1; ++b) {
+    look(b);
+    sum += (int64_t)tiles * steps;
+  }
+  const int64_t total = block_sum(sum, before) * a.Hkv;
+  const int64_t size = total / a.blocks + 1 > a.least ? total / a.blocks + 1 : a.least;
+  auto parts_of_tile = [&]() { return steps > 0 ? (int)((steps + size - 1) / size) : 1; };
+  if (each > 1 || b0 >= b1) {
+    sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      look(b);
+      sum += (int64_t)tiles * parts_of_tile();
+    }
+  } else {
+    sum = (int64_t)tiles * parts_of_tile();
+  }
+  if (threadIdx.x == 0) s_work->any = false;
+  block_sum(sum, before);
+  if (y >= before && y < before + sum) {
+    for (int b = b0; b < b1; ++b) {
+      if (each > 1) look(b);
+      const int parts = parts_of_tile();
+      const int64_t here = (int64_t)tiles * parts;
+      if (y < before + here) {
+        const int tile = (int)((y - before) / parts);
+        Work t;
+        t.q0 = q0;
+        t.b = b;
+        t.n = n;
+        t.row0 = (tiles - 1 - tile) * R;
+        t.part = (int)(y - before) - tile * parts;
+        t.parts = parts;
+        t.first = y - t.part;
+        t.hk = 0;
+        t.any = true;
+        *s_work = t;
+        break;
+      }
+      before += here;
+    }
+  }
+  __syncthreads();
+  return *s_work;
+}
+
+template <int R, int STEP, int THREADS>
+__device__ __forceinline__ Work pick_work(const AttendArgs& a, int64_t* s_sum, Work* s_work) {
+  const unsigned x = blockIdx.x, y = x / (unsigned)a.Hkv;  // heads side by side: each to its own XCD's cache
+  Work t = a.blocks > 0 ? pick_part<R, STEP, THREADS>(a, y, s_sum, s_work) : pick_tile(a, y, R);
+  t.hk = (int)(x - y * (unsigned)a.Hkv);
+  t.b = __builtin_amdgcn_readfirstlane(t.b);
+  t.n = __builtin_amdgcn_readfirstlane(t.n);
+  t.row0 = __builtin_amdgcn_readfirstlane(t.row0);
+  t.part = __builtin_amdgcn_readfirstlane(t.part);
+  t.parts = __builtin_amdgcn_readfirstlane(t.parts);
+  return t;
+}
+
+// Tokens [lo, hi) that some of the rows see, which stand at pos_min .. pos_max.
+struct Span {
+  int lo, hi;
+};
+__device__ __forceinline__ Span span_of(const AttendArgs& a, int b, int pos_min, int pos_max) {
+  Span s;
+  s.hi = pos_max + 1;
+  const int64_t reach = (int64_t)a.width << a.shift;
+  if (s.hi > reach) s.hi = (int)reach;
+  s.lo = a.window > 0 && pos_min - a.window + 1 > 0 ? pos_min - a.window + 1 : 0;
+  if (b >= a.B || s.hi < s.lo) s.hi = s.lo;
+  return s;
+}
+
+// The lane's query row as operands: KS pieces of 8 values, `stride` apart from q on; what its scores
+// have to be multiplied by; and for codes, its groups' sums (this lane's part of them).
+template <class T, int KS, int STRIDE, int G, class Frag>
+__device__ __forceinline__ float load_query(const T* q, float scale_log2, Frag (&qf)[KS][kParts<T>], float (&sums)[G]) {
+  float v[KS][8], top = 0.f;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    load_values<T, 8>(q + STRIDE * k, v[k]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = max_of(top, __builtin_fabsf(v[k][e]));
+  }
+  int e2 = 0;
+  if constexpr (__is_same(T, __bf16)) {
+    top = STRIDE == 32 ? quad_max(top) : pair_max(top);
+    e2 = top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[k][e] = __builtin_amdgcn_ldexpf(v[k][e], -e2);
+  }
+#pragma unroll
+  for (int g = 0; g < G; ++g) sums[g] = 0.f;
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    parts_of(v[k], qf[k]);
+    if constexpr (kCodes<T>)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sums[k * STRIDE / kKv4Group] += v[k][e];
+  }
+  return __builtin_amdgcn_ldexpf(scale_log2, e2);
+}
+
+// This block's part is written: true in the block that is the last of its tile's, which then sees
+// the others' parts.
+__device__ __forceinline__ bool last_part(const AttendArgs& a, const Work& w, int* s_last) {
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    int* count = a.done + w.first * a.Hkv + w.hk;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
+    const int before = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (before == w.parts - 1) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    *s_last = before == w.parts - 1;
+  }
+  __syncthreads();
+  if (!*s_last) return false;
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+  return true;
+}
+
+// ---- few rows --------------------------------------------------------------------------------
+// Whether registers hold two steps' codes besides the queries and results, and the waves a SIMD
+// that they leave room for.
+template <class T, int D, int RT>
+constexpr bool kFewAhead = D < 256;
+template <class T, int D, int RT>
+constexpr int kFewWaves = (kCodes<T> ? (RT == 2 ? 1 : 2) : (RT == 2 ? 2 : 3)) + (D == 64 ? 1 : 0) - (D == 256 ? 1 : 0);
+
 template <class T, int D, int RT, int NW>
-__global__ __launch_bounds__(64 * NW) void k_kv4_attend(AttendArgs a) {
+__global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(AttendArgs a) {
   using O = Ops<T>;
   typedef typename O::Frag Frag;
-  constexpr int G = D / kKv4Group, KS = D / 32, R = 16 * RT, W = 2 * G;
-  constexpr bool kHalf = sizeof(T) == 2;
+  constexpr int G = D / kKv4Group, KS = D / 32, R = 16 * RT, W = 2 * G, NP = kParts<T>;
+  constexpr int KW = kCodes<T> ? 4 * G : G;  // dwords of key scales: the scores' four tokens, or the operand's own
   __shared__ float s_o[NW][16][D + 4];
   __shared__ float2 s_ml[NW][16];
+  __shared__ int64_t s_sum[NW];
+  __shared__ Work s_work;
+  __shared__ int s_last;
   const int lane = threadIdx.x & 63, n = lane & 15, qq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int hk = blockIdx.y;
-  const Tile tile = find_tile(a, blockIdx.x, R);
+  const Work tile = pick_work<R, 32, 64 * NW>(a, s_sum, &s_work);
   if (!tile.any) return;
-  const int rows = tile.n * a.grp;
-  int ctx = tile.b < a.B ? a.context[tile.b] : 0;
-  ctx = ctx < 0 ? 0 : ctx < (1 << 30) ? ctx : 1 << 30;
-  const int past = ctx - tile.n;  // position of the first new token
+  const int hk = tile.hk, rows = tile.n * a.grp;
+  const int past = context_of(a, tile.b) - tile.n;  // position of the first new token
   const int r_last = tile.row0 + R - 1 < rows ? tile.row0 + R - 1 : rows - 1;
   const int pos_min = past + tile.row0 / a.grp, pos_max = past + r_last / a.grp;
-  // tokens [lo, hi) are seen by some row of the tile
-  int hi = pos_max + 1;
-  const int64_t reach = (int64_t)a.width << a.shift;
-  if (hi > reach) hi = (int)reach;
-  int lo = a.window > 0 && pos_min - a.window + 1 > 0 ? pos_min - a.window + 1 : 0;
-  if (tile.b >= a.B || hi < lo) hi = lo;
+  const Span span = span_of(a, tile.b, pos_min, pos_max);
+  const int lo = span.lo, hi = span.hi;
 
   // queries: the lane's row, values d = 32 i + 8 qq + (0..7)
-  Frag qf[RT][KS];
-  float rs[RT];
+  Frag qf[RT][KS][NP];
+  float rs[RT], qs[RT][G];
   int pos[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int row = tile.row0 + rt * 16 + n;
-    const bool in = row < rows;
-    const int i = (in ? row : rows - 1) / a.grp;
-    const int head = hk * a.grp + (in ? row : rows - 1) - i * a.grp;
+    int row = tile.row0 + rt * 16 + n;
+    if (row >= rows) row = rows - 1;
+    const int i = row / a.grp, head = hk * a.grp + row - i * a.grp;
     pos[rt] = past + i;
-    const T* q = static_cast<const T*>(a.q) + (tile.q0 + i) * a.ldq_t + head * a.ldq_h + 8 * qq;
-    float v[KS][8];
-    float top = 0.f;
+    rs[rt] = load_query<T, KS, 32, G>(static_cast<const T*>(a.q) + (tile.q0 + i) * a.ldq_t + head * a.ldq_h + 8 * qq,
+                                      a.scale_log2, qf[rt], qs[rt]);
+    if constexpr (kCodes<T>)
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      load_values<T, 8>(q + 32 * k, v[k]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) top = max_of(top, __builtin_fabsf(v[k][e]));
-    }
-    rs[rt] = a.scale_log2;
-    if constexpr (kHalf) {
-      int e2 = 0;
-      if constexpr (__is_same(T, __bf16)) {
-        top = quad_max(top);
-        e2 = top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
-        rs[rt] = __builtin_amdgcn_ldexpf(a.scale_log2, e2);
-      }
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) qf[rt][k][e] = static_cast<_Float16>(__builtin_amdgcn_ldexpf(v[k][e], -e2));
-    } else {
-#pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) qf[rt][k].v[e] = v[k][e];
-    }
+      for (int g = 0; g < G; ++g) qs[rt][g] = quad_sum(qs[rt][g]);
   }
 
   // this block's steps of 32 tokens, of which the wave takes every NW-th
   const int first = lo >> 5, steps = ((hi + 31) >> 5) - first;
-  const int s0 = first + (int)((int64_t)steps * blockIdx.z / a.splits);
-  const int s1 = first + (int)((int64_t)steps * (blockIdx.z + 1) / a.splits);
+  const int s0 = first + (int)((int64_t)steps * tile.part / tile.parts);
+  const int s1 = first + (int)((int64_t)steps * (tile.part + 1) / tile.parts);
 
   const Kv4Layout L(a.P, D);
   const int64_t block_bytes = L.bytes();
   const int* table = a.tables + (int64_t)(tile.b < a.B ? tile.b : 0) * a.ld_table;
 
   f32x4 o[RT][G][4];
-  float m[RT], l[RT];
+  float m[RT], l[RT], ol[RT][G];  // ol: codes' sum of p lo
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -__builtin_inff();
     l[rt] = 0.f;
 #pragma unroll
-    for (int g = 0; g < G; ++g)
+    for (int g = 0; g < G; ++g) {
+      ol[rt][g] = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[rt][g][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
   }
 
   struct Raw {
-    uint32_t k[2][KS], ks[2][G], v[2][W], vs[2][G][4];
-    bool bad[2];
+    uint32_t k[2][KS], ks[2][KW], v[2][W], vs[2][G][4];
   };
-  int ids = 0;
-  // the pages of the wave's next 32 steps: lane l holds that of step l / 2, tokens 16 (l & 1)
-  auto load_ids = [&](int it) {
-    const int64_t t = (int64_t)(s0 + wave + NW * (it + (lane >> 1))) * 32 + 16 * (lane & 1);
-    ids = t < hi ? table[t >> a.shift] : -1;
-  };
-  auto load = [&](int it, Raw& r) {
-    if ((it & 31) == 0) load_ids(it);
+  // lane l holds the page of the wave's step l / 2, tokens 16 (l & 1), of a run of 32 steps
+  int ids = -1;
+  uint64_t gone = 0;  // those that are no page
+  auto load = [&](int at, int step, Raw& r) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int t = (s0 + wave + NW * it) * 32 + 16 * h;
-      const int id = __builtin_amdgcn_readlane(ids, 2 * (it & 31) + h);
-      r.bad[h] = id < 0 || id >= a.pages;
-      const uint8_t* block = a.cache + ((int64_t)(r.bad[h] ? 0 : id) * a.Hkv + hk) * block_bytes;
+      const int t = step * 32 + 16 * h;
+      const int id = __builtin_amdgcn_readlane(ids, 2 * at + h);
+      const uint8_t* block = a.cache + ((int64_t)id * a.Hkv + hk) * block_bytes;
       const int tl = t & (a.P - 1);
       const uint8_t* kp = block + (tl + n) * (D / 2) + qq * (KS * 4);
-      const uint8_t* sp = block + L.k_scales() + (tl + n) * (G * 4);
+      const uint8_t* sp = block + L.k_scales() + (tl + (kCodes<T> ? 4 * qq : n)) * (G * 4);
       const uint8_t* vp = block + L.v_codes() + (tl / 4 + qq) * (32 * W * 4 / 2) + n * (W * 4);
       const uint8_t* wp = block + L.v_scales() + (tl / 4 + qq) * (G * 16);
       __builtin_memcpy(r.k[h], __builtin_assume_aligned(kp, KS * 4 < 16 ? KS * 4 : 16), KS * 4);
-      __builtin_memcpy(r.ks[h], __builtin_assume_aligned(sp, G * 4), G * 4);
+      __builtin_memcpy(r.ks[h], __builtin_assume_aligned(sp, KW * 4 < 16 ? KW * 4 : 16), KW * 4);
       __builtin_memcpy(r.v[h], __builtin_assume_aligned(vp, W * 4 < 16 ? W * 4 : 16), W * 4);
       __builtin_memcpy(r.vs[h], __builtin_assume_aligned(wp, 16), G * 16);
     }
   };
-
-  Raw cur, next;
-  const int its = s1 - s0 > wave ? (s1 - s0 - wave + NW - 1) / NW : 0;
-  if (its > 0) load(0, cur);
-  for (int it = 0; it < its; ++it) {
-    if (it + 1 < its) load(it + 1, next);
-    const int t0 = (s0 + wave + NW * it) * 32;
-    const bool edge = t0 + 31 > pos_min || t0 + 32 > hi || t0 < lo || (a.window > 0 && t0 <= pos_max - a.window) ||
-                      cur.bad[0] || cur.bad[1];
+  auto step_of = [&](int step, int at, Raw& cur) {
+    const int t0 = step * 32;
+    const int bad = (int)(gone >> (2 * at)) & 3;
+    const bool edge = t0 + 31 > pos_min || t0 + 32 > hi || t0 < lo || (a.window > 0 && t0 <= pos_max - a.window) || bad;
     if (edge) {  // tokens that no row sees take no part whatever their page holds
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int t = t0 + 16 * h + 4 * qq + 2 * c;
-          const uint32_t keep = (!cur.bad[h] && t >= lo && t < hi ? 0xffffu : 0u) |
-                                (!cur.bad[h] && t + 1 >= lo && t + 1 < hi ? 0xffff0000u : 0u);
+          const bool ok = !(bad >> h & 1);
+          const uint32_t keep = (ok && t >= lo && t < hi ? 0xffffu : 0u) | (ok && t + 1 >= lo && t + 1 < hi ? 0xffff0000u : 0u);
 #pragma unroll
           for (int g = 0; g < G; ++g) {
             cur.vs[h][g][c] &= keep;
@@ -305,101 +495,174 @@ __global__ __launch_bounds__(64 * NW) void k_kv4_attend(AttendArgs a) {
           }
         }
     }
-    f32x4 sc[RT][2];
+    float x[RT][8];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
+      if constexpr (kCodes<T>) {
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) sc[rt][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        const Frag kf = O::key(cur.k[h][k], cur.ks[h][k / 2]);
+          for (int rt = 0; rt < RT; ++rt) x[rt][4 * h + e] = 0.f;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) sc[rt][h] = O::mma(kf, qf[rt][k], sc[rt][h]);
+        for (int g = 0; g < G; ++g) {
+          f32x4 sc[RT];
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 2 * g; k < 2 * g + 2; ++k) {
+            const Frag kf = O::key(cur.k[h][k], 0);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+              for (int p = NP - 1; p >= 0; --p) sc[rt] = O::mma(kf, qf[rt][k][p], sc[rt]);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const uint32_t sl = cur.ks[h][r * G + g];
+            const float s = f16_bits_to_f32((uint16_t)sl), z = f16_bits_to_f32((uint16_t)(sl >> 16));
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+              x[rt][4 * h + r] = __builtin_fmaf(s, sc[rt][r], __builtin_fmaf(z, qs[rt][g], x[rt][4 * h + r]));
+          }
+        }
+      } else {
+        f32x4 sc[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) sc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const Frag kf = O::key(cur.k[h][k], cur.ks[h][k / 2]);
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) sc[rt] = O::mma(kf, qf[rt][k][0], sc[rt]);
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[rt][4 * h + r] = sc[rt][r];
       }
     }
-    Frag pf[RT];
+    float p[RT][8];
+    Frag pf[RT][NP];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float x[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = sc[rt][e >> 2][e & 3] * rs[rt];
       if (edge) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int t = t0 + 16 * (e >> 2) + 4 * qq + (e & 3);
-          const bool see = t <= pos[rt] && t < hi && (a.window <= 0 || t > pos[rt] - a.window) && !cur.bad[e >> 2];
-          x[e] = see ? x[e] : -__builtin_inff();
+          const bool see = t <= pos[rt] && t < hi && (a.window <= 0 || t > pos[rt] - a.window) && !(bad >> (e >> 2) & 1);
+          x[rt][e] = see ? x[rt][e] : -__builtin_inff();
         }
       }
-      float top = x[0];
+      float top = x[rt][0] *= rs[rt];
 #pragma unroll
-      for (int e = 1; e < 8; ++e) top = max_of(top, x[e]);
-      top = max_of(m[rt], quad_max(top));
-      const float base = top == -__builtin_inff() ? 0.f : top;
-      if (__any(top > m[rt])) {
-        const float f = __builtin_amdgcn_exp2f(m[rt] - base);
+      for (int e = 1; e < 8; ++e) top = fmaxf(top, x[rt][e] *= rs[rt]);
+      top = quad_max(top);
+      if (__any(top > m[rt] + kSlack)) {
+        const float to = max_of(m[rt], top);
+        const float f = to == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[rt] - to);
         l[rt] *= f;
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < G; ++g) {
+          if constexpr (kCodes<T>) ol[rt][g] *= f;
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[rt][g][j] *= f;
-        m[rt] = top;
+        }
+        m[rt] = to;
       }
-      float p[8], sum = 0.f;
+      const float base = m[rt] == -__builtin_inff() ? 0.f : m[rt];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(x[e] - base);
-        sum += p[e];
+        p[rt][e] = __builtin_amdgcn_exp2f(x[rt][e] - base);
+        l[rt] += p[rt][e];
       }
-      l[rt] += sum;
-      pf[rt] = O::weights(p);
+      if constexpr (!kCodes<T>) parts_of(p[rt], pf[rt]);
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       uint32_t u[4], s[4], z[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // token pairs (0, 1), (2, 3) of both tiles' units
-        const int h = i >> 1, c = i & 1;
-        if constexpr (G == 1) {
-          u[i] = cur.v[h][c];
-        } else {
-          const uint32_t w0 = cur.v[h][(2 * c) * (G / 2) + g / 2], w1 = cur.v[h][(2 * c + 1) * (G / 2) + g / 2];
-          u[i] = __builtin_amdgcn_perm(w1, w0, g & 1 ? 0x07060302u : 0x05040100u);
-        }
-        s[i] = cur.vs[h][g][c];
-        z[i] = cur.vs[h][g][2 + c];
+        u[i] = cur.v[i >> 1][2 * g + (i & 1)];
+        s[i] = cur.vs[i >> 1][g][i & 1];
+        z[i] = cur.vs[i >> 1][g][2 + (i & 1)];
       }
+      if constexpr (kCodes<T>) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const Frag vf = O::val(u, s, z, j);
+        for (int rt = 0; rt < RT; ++rt) {
+          float w[8];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) o[rt][g][j] = O::mma(vf, pf[rt], o[rt][g][j]);
+          for (int e = 0; e < 8; ++e) {
+            const int up = 16 * (e & 1);
+            w[e] = p[rt][e] * f16_bits_to_f32((uint16_t)(s[e >> 1] >> up));
+            ol[rt][g] = __builtin_fmaf(p[rt][e], f16_bits_to_f32((uint16_t)(z[e >> 1] >> up)), ol[rt][g]);
+          }
+          parts_of(w, pf[rt]);
+        }
+      }
+      auto product = [&](const Frag& vf, int j) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+          for (int q = NP - 1; q >= 0; --q) o[rt][g][j] = O::mma(vf, pf[rt][q], o[rt][g][j]);
+      };
+      product(O::template val<0>(u, s, z), 0);
+      product(O::template val<1>(u, s, z), 1);
+      product(O::template val<2>(u, s, z), 2);
+      product(O::template val<3>(u, s, z), 3);
+    }
+  };
+
+  const int its = s1 - s0 > wave ? (s1 - s0 - wave + NW - 1) / NW : 0;
+  for (int it0 = 0; it0 < its; it0 += 32) {
+    const int run = its - it0 < 32 ? its - it0 : 32;
+    const int base = s0 + wave + NW * it0;
+    {
+      const int64_t t = (int64_t)(base + NW * (lane >> 1)) * 32 + 16 * (lane & 1);
+      ids = (lane >> 1) < run && t < hi ? table[t >> a.shift] : -1;
+      const bool bad = ids < 0 || ids >= a.pages;
+      gone = __ballot(bad);
+      if (bad) ids = 0;  // in bounds, and not seen
+    }
+    Raw ra;
+    auto fetch = [&](int i, Raw& r) {
+      i = i < run ? i : run - 1;
+      load(i, base + NW * i, r);
+    };
+    fetch(0, ra);
+    if constexpr (kFewAhead<T, D, RT>) {
+      // the next steps' loads are under way while one is computed; past the end the last is read again
+      Raw rb;
+      fetch(1, rb);
+      for (int i = 0;; i += 2) {
+        step_of(base + NW * i, i, ra);
+        if (i + 1 >= run) break;
+        fetch(i + 2, ra);
+        step_of(base + NW * (i + 1), i + 1, rb);
+        if (i + 2 >= run) break;
+        fetch(i + 3, rb);
+      }
+    } else {
+      for (int i = 0;; ++i) {
+        step_of(base + NW * i, i, ra);
+        if (i + 1 >= run) break;
+        fetch(i + 1, ra);
       }
     }
-    cur = next;
   }
 
-  // join the waves, 16 rows at a time
+  // join the waves, 16 rows at a time; then, in a tile's last block, its parts the same way
   constexpr int TPR = 64 * NW / 16, C = D / TPR;  // threads a row, values a thread
   const int row_of = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * C;
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const float sum = quad_sum(l[rt]);
-    if (rt) __syncthreads();
-    if (qq == 0) s_ml[wave][n] = {m[rt], sum};
-#pragma unroll
-    for (int g = 0; g < G; ++g)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const f32x4 w = {o[rt][g][0][r], o[rt][g][1][r], o[rt][g][2][r], o[rt][g][3][r]};
-        *reinterpret_cast<f32x4*>(&s_o[wave][n][64 * g + 16 * qq + 4 * r]) = w;
-      }
+  const int64_t tile0 = (tile.first * a.Hkv + hk) * (int64_t)R, tile_step = (int64_t)a.Hkv * R;
+  auto join = [&](int rt, float (&v)[C], float& top, float& all) {
     __syncthreads();
-    float top = -__builtin_inff();
+    top = -__builtin_inff();
 #pragma unroll
     for (int w = 0; w < NW; ++w) top = max_of(top, s_ml[w][row_of].x);
     const float base = top == -__builtin_inff() ? 0.f : top;
-    float all = 0.f, v[C] = {};
+    all = 0.f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) v[c] = 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const float2 ml = s_ml[w][row_of];
@@ -408,93 +671,519 @@ __global__ __launch_bounds__(64 * NW) void k_kv4_attend(AttendArgs a) {
 #pragma unroll
       for (int c = 0; c < C; ++c) v[c] = __builtin_fmaf(s_o[w][row_of][d0 + c], f, v[c]);
     }
+    __syncthreads();
+  };
+  auto finish = [&](int rt, float (&v)[C], float all) {
     const int row = tile.row0 + rt * 16 + row_of;
-    if (row < rows) {
-      const int i = row / a.grp;
-      const int64_t at = (tile.q0 + i) * ((int64_t)a.Hkv * a.grp) + hk * a.grp + row - i * a.grp;
-      if (a.splits == 1) {
-        const float inv = all == 0.f ? 0.f : 1.f / all;
+    if (row >= rows) return;
+    const int i = row / a.grp;
+    const int64_t at = (tile.q0 + i) * ((int64_t)a.Hkv * a.grp) + hk * a.grp + row - i * a.grp;
+    const float inv = all == 0.f ? 0.f : 1.f / all;
 #pragma unroll
-        for (int c = 0; c < C; ++c) v[c] *= inv;
-        store_values<T, C>(static_cast<T*>(a.out) + at * D + d0, v);
-      } else {
-        const int64_t pa = (int64_t)blockIdx.z * a.T * a.Hkv * a.grp + at;
-        store_values<float, C>(a.part_o + pa * D + d0, v);
-        if (d0 == 0) a.part_ml[pa] = {top, all};
+    for (int c = 0; c < C; ++c) v[c] *= inv;
+    store_values<T, C>(static_cast<T*>(a.out) + at * D + d0, v);
+  };
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const float sum = quad_sum(l[rt]);
+    if (qq == 0) s_ml[wave][n] = {m[rt], sum};
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float add = kCodes<T> ? quad_sum(ol[rt][g]) : 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        f32x4 w = {o[rt][g][0][r], o[rt][g][1][r], o[rt][g][2][r], o[rt][g][3][r]};
+        if constexpr (kCodes<T>) w += add;
+        *reinterpret_cast<f32x4*>(&s_o[wave][n][64 * g + 16 * qq + 4 * r]) = w;
       }
     }
+    float v[C], top, all;
+    join(rt, v, top, all);
+    if (tile.parts == 1) {
+      finish(rt, v, all);
+    } else if (tile.row0 + rt * 16 + row_of < rows) {
+      const int64_t at = tile0 + tile.part * tile_step + rt * 16 + row_of;
+      store_values<float, C>(a.part_o + at * D + d0, v);
+      if (d0 == 0) a.part_ml[at] = {top, all};
+    }
+  }
+  if (tile.parts == 1 || !last_part(a, tile, &s_last)) return;
+  constexpr int RI = 256 / D, RN = 16 / RI, LR = 64 / RI;  // rows a pass of four values a lane, passes, lanes a row
+#pragma unroll 1
+  for (int rt = 0; rt < RT; ++rt) {
+    const int live = rows - tile.row0 - rt * 16;  // rows of these 16 that exist
+    float2 ml[RN];
+    f32x4 acc[RN];
+#pragma unroll
+    for (int i = 0; i < RN; ++i) {
+      ml[i] = {-__builtin_inff(), 0.f};
+      acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll 2
+    for (int c = wave; c < tile.parts; c += NW) {
+      const int64_t at = tile0 + c * tile_step + rt * 16 + lane / LR;
+#pragma unroll
+      for (int i = 0; i < RN; ++i) {
+        if (i * RI + lane / LR >= live) continue;
+        const float2 pm = a.part_ml[at + i * RI];
+        const f32x4 po = *reinterpret_cast<const f32x4*>(a.part_o + (at + i * RI) * D + (lane % LR) * 4);
+        const float to = max_of(ml[i].x, pm.x), base = to == -__builtin_inff() ? 0.f : to;
+        const float f0 = __builtin_amdgcn_exp2f(ml[i].x - base), f1 = __builtin_amdgcn_exp2f(pm.x - base);
+        ml[i] = {to, ml[i].y * f0 + pm.y * f1};
+        acc[i] = acc[i] * f0 + po * f1;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < RN; ++i) {
+      const int row = i * RI + lane / LR;
+      if (lane % LR == 0) s_ml[wave][row] = ml[i];
+      *reinterpret_cast<f32x4*>(&s_o[wave][row][(lane % LR) * 4]) = acc[i];
+    }
+    float v[C], top, all;
+    join(rt, v, top, all);
+    finish(rt, v, all);
   }
 }
 
-// A wave a row: the splits' maxima and sums first, then their results with weights.
+// ---- many rows -------------------------------------------------------------------------------
+// 64 tokens (32 of heads of 256) unpacked in LDS, each eight values along a product's sum in 16
+// bytes, in the order in which v_mfma_f32_32x32x16 takes them:
+//   keys   [token / 32][d / 16][d / 8 & 1][token & 31]
+//   values [d' / 32][token / 16][h][d' & 31]: d' = 64 g + 16 j + m of value 64 g + 4 m + j, and the
+//          tokens 16 s + 4 h + (0..3), 16 s + 8 + 4 h + (0..3), which is where the scores' result
+//          leaves the weights: these never cross lanes.
 template <class T, int D>
-__global__ __launch_bounds__(256) void k_kv4_join(const float* part_o, const float2* part_ml, int64_t rows, int splits,
-                                                  T* out) {
-  constexpr int C = D / 64;
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= rows) return;
-  float2 ml = {-__builtin_inff(), 0.f};
-  if (lane < splits) ml = part_ml[lane * rows + row];  // at most 64 splits
-  const float top = wave_max(ml.x);
-  const float base = top == -__builtin_inff() ? 0.f : top;
-  const float f = __builtin_amdgcn_exp2f(ml.x - base);
-  const float all = wave_sum_dpp(ml.y * f);
-  float v[C] = {};
-  for (int s = 0; s < splits; ++s) {
-    const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s));
-    float x[C];
-    load_values<float, C>(part_o + (s * rows + row) * D + lane * C, x);
+struct RowsTile {
+  static constexpr int TT = D == 256 ? 32 : 64, U = TT / 32, G = D / kKv4Group;
+  static constexpr int kChunks = TT * D / 8;  // of 16 bytes, for keys and for values
+  typedef typename Ops<T>::Frag Frag;
+  Frag k[kChunks], v[kChunks];
+  float ks[kCodes<T> ? G : 1][kCodes<T> ? TT : 1], kl[kCodes<T> ? G : 1][kCodes<T> ? TT : 1];
+  float vs[kCodes<T> ? G : 1][kCodes<T> ? TT : 1], vl[kCodes<T> ? G : 1][kCodes<T> ? TT : 1];
+};
+
+template <class T, int D>
+__global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) void k_attend_rows(AttendArgs a) {
+  using O = Ops<T>;
+  typedef typename O::Frag Frag;
+  typedef RowsTile<T, D> Tile;
+  constexpr int G = D / kKv4Group, KS = D / 16, DT = D / 32, NP = kParts<T>, TT = Tile::TT, U = Tile::U, R = 128;
+  constexpr int UB = kCodes<T> ? 1 : U;       // halves of 32 tokens that share a softmax step (registers)
+  constexpr int C = Tile::kChunks / 256;      // chunks of keys (and of values) a thread unpacks
+  constexpr int KG = D == 64 ? 1 : 2;         // groups that a thread's dwords of keys belong to
+  extern __shared__ __attribute__((aligned(16))) char s_mem[];
+  Tile* s_tile = reinterpret_cast<Tile*>(s_mem);  // two
+  __shared__ int64_t s_sum[4];
+  __shared__ Work s_work;
+  __shared__ int s_last;
+  const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Work tile = pick_work<R, TT, 256>(a, s_sum, &s_work);
+  if (!tile.any) return;
+  const int hk = tile.hk, rows = tile.n * a.grp;
+  const int past = context_of(a, tile.b) - tile.n;
+  const int r_last = tile.row0 + R - 1 < rows ? tile.row0 + R - 1 : rows - 1;
+  const Span span = span_of(a, tile.b, past + tile.row0 / a.grp, past + r_last / a.grp);
+  const int lo = span.lo, hi = span.hi;
+
+  // the wave's 32 rows, and the positions between which they stand
+  const int wrow = tile.row0 + 32 * wave;
+  const bool busy = wrow < rows;
+  const int wlast = wrow + 31 < rows ? wrow + 31 : rows - 1;
+  const int pos_min = past + (busy ? wrow : wlast) / a.grp, pos_max = past + wlast / a.grp;
+  const int row = wrow + n < rows ? wrow + n : rows - 1;
+  const int qi = row / a.grp, head = hk * a.grp + row - qi * a.grp;
+  const int pos = past + qi;
+  Frag qf[KS][NP];
+  float qs[G];
+  const float rs = load_query<T, KS, 16, G>(static_cast<const T*>(a.q) + (tile.q0 + qi) * a.ldq_t + head * a.ldq_h + 8 * h,
+                                            a.scale_log2, qf, qs);
+  if constexpr (kCodes<T>)
 #pragma unroll
-    for (int c = 0; c < C; ++c) v[c] = __builtin_fmaf(x[c], w, v[c]);
-  }
-  const float inv = all == 0.f ? 0.f : 1.f / all;
+    for (int g = 0; g < G; ++g) qs[g] = pair_sum(qs[g]);
+
+  const int first = lo / TT, steps = (hi + TT - 1) / TT - first;
+  const int s0 = first + (int)((int64_t)steps * tile.part / tile.parts);
+  const int s1 = first + (int)((int64_t)steps * (tile.part + 1) / tile.parts);
+  const Kv4Layout L(a.P, D);
+  const int64_t block_bytes = L.bytes();
+  const int* table = a.tables + (int64_t)(tile.b < a.B ? tile.b : 0) * a.ld_table;
+
+  // ---- unpacking: what a thread takes of a step's tokens
+  // keys: token kt of the step, dwords kq D/32 + k0 .. + C - 1
+  // values: units va and va + 2 of four tokens, words m of group vg, nibbles j0 .. j0 + C - 1
+  const int n16 = lane & 15, qq = lane >> 4;
+  const int kt = D == 256 ? 16 * (wave & 1) + n16 : 16 * wave + n16, k0 = D == 256 ? 4 * (wave >> 1) : 0;
+  const int vt = D == 256 ? 0 : wave >> 1, va = 8 * vt + 4 * (qq >> 1) + (qq & 1);
+  const int vg = D == 256 ? wave : D == 128 ? wave & 1 : 0, j0 = D == 64 ? 2 * (wave & 1) : 0;
+  struct Raw {
+    uint32_t k[C], ks[KG], v[4], vs[2][4];
+  };
+  // lane l holds the page of tokens 16 l .. of a run of 1024 tokens
+  constexpr int RUN = 1024 / TT, E = TT / 16;
+  int ids = 0;
+  uint64_t gone = 0;
+  auto load = [&](int at, int step, Raw& r) {
+    auto block_of = [&](int sub) {
+      return a.cache + ((int64_t)__builtin_amdgcn_readlane(ids, E * at + sub) * a.Hkv + hk) * block_bytes;
+    };
+    {
+      const int sub = D == 256 ? wave & 1 : wave;
+      const uint8_t* block = block_of(sub);
+      const int tl = ((step * TT + 16 * sub) & (a.P - 1)) + n16;
+      const uint8_t* kp = block + tl * (D / 2) + (qq * (D / 32) + k0) * 4;
+      __builtin_memcpy(r.k, __builtin_assume_aligned(kp, C * 4), C * 4);
+      const uint8_t* sp = block + L.k_scales() + (tl * G + k0 / 2) * 4;
+      __builtin_memcpy(r.ks, __builtin_assume_aligned(sp, KG * 4), KG * 4);
+    }
 #pragma unroll
-  for (int c = 0; c < C; ++c) v[c] *= inv;
-  if constexpr (C * sizeof(T) >= 4) {
-    store_values<T, C>(out + row * D + lane * C, v);
-  } else {
-    out[row * D + lane] = from_f32<T>(v[0]);
+    for (int x = 0; x < 2; ++x) {  // units va and va + 2 of a 32-token half: one 16-token page part each pair of lanes
+      const int sub0 = 2 * vt + (qq >> 1);
+      const int id = __shfl(ids, E * at + sub0, 64);
+      const uint8_t* block = a.cache + ((int64_t)id * a.Hkv + hk) * block_bytes;
+      const int tl = ((step * TT + 16 * sub0) & (a.P - 1)) / 4 + (qq & 1) + 2 * x;
+      const uint8_t* vp = block + L.v_codes() + ((tl * 16 + n16) * G + vg) * 8;
+      __builtin_memcpy(r.v + 2 * x, __builtin_assume_aligned(vp, 8), 8);
+      const uint8_t* wp = block + L.v_scales() + (tl * G + vg) * 16;
+      __builtin_memcpy(r.vs[x], __builtin_assume_aligned(wp, 16), 16);
+    }
+  };
+  auto unpack = [&](int at, int step, Raw& r, Tile& t) {
+    // tokens that no row sees take no part whatever their page holds
+    const int t0 = step * TT;
+    const int bad = (int)(gone >> (E * at)) & ((1 << E) - 1);
+    if (t0 < lo || t0 + TT > hi || bad) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int tok = t0 + 4 * (va + 2 * x) + 2 * c;
+          const bool ok = !(bad >> (2 * vt + (qq >> 1)) & 1);
+          const uint32_t keep = (ok && tok >= lo && tok < hi ? 0xffffu : 0u) | (ok && tok + 1 >= lo && tok + 1 < hi ? 0xffff0000u : 0u);
+          r.vs[x][c] &= keep;
+          r.vs[x][2 + c] &= keep;
+        }
+    }
+    Frag* kd = t.k + ((kt >> 5) * KS) * 64 + (kt & 31) + (qq & 1) * 32;
+#pragma unroll
+    for (int c = 0; c < C; ++c) kd[(2 * (k0 + c) + (qq >> 1)) * 64] = O::key(r.k[c], r.ks[c / 2]);
+    const uint32_t s[4] = {r.vs[0][0], r.vs[0][1], r.vs[1][0], r.vs[1][1]};
+    const uint32_t z[4] = {r.vs[0][2], r.vs[0][3], r.vs[1][2], r.vs[1][3]};
+    Frag* vd = t.v + (2 * vg * (TT / 16) + 2 * vt + (qq >> 1)) * 64 + (qq & 1) * 32 + n16;
+    if constexpr (D == 64) {
+      if (j0 == 0) {
+        vd[0] = O::template val<0>(r.v, s, z);
+        vd[16] = O::template val<1>(r.v, s, z);
+      } else {
+        vd[(TT / 16) * 64] = O::template val<2>(r.v, s, z);
+        vd[(TT / 16) * 64 + 16] = O::template val<3>(r.v, s, z);
+      }
+    } else {
+      vd[0] = O::template val<0>(r.v, s, z);
+      vd[16] = O::template val<1>(r.v, s, z);
+      vd[(TT / 16) * 64] = O::template val<2>(r.v, s, z);
+      vd[(TT / 16) * 64 + 16] = O::template val<3>(r.v, s, z);
+    }
+    if constexpr (kCodes<T>) {
+      if (qq == 0) {
+#pragma unroll
+        for (int g = 0; g < KG; ++g) {
+          t.ks[k0 / 2 + g][kt] = f16_bits_to_f32((uint16_t)r.ks[g]);
+          t.kl[k0 / 2 + g][kt] = f16_bits_to_f32((uint16_t)(r.ks[g] >> 16));
+        }
+      }
+      if (n16 == 0) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            t.vs[vg][4 * (va + 2 * x) + e] = f16_bits_to_f32((uint16_t)(r.vs[x][e >> 1] >> (16 * (e & 1))));
+            t.vl[vg][4 * (va + 2 * x) + e] = f16_bits_to_f32((uint16_t)(r.vs[x][2 + (e >> 1)] >> (16 * (e & 1))));
+          }
+      }
+    }
+  };
+
+  f32x16 o[DT];
+  float m = -__builtin_inff(), l = 0.f, ol[G];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+#pragma unroll
+  for (int g = 0; g < G; ++g) ol[g] = 0.f;
+
+  auto compute = [&](int at, int step, const Tile& t) {
+    const int t0 = step * TT;
+    const int bad = (int)(gone >> (E * at)) & ((1 << E) - 1);
+    if (!busy || t0 > pos_max || (a.window > 0 && t0 + TT <= pos_min - a.window + 1)) return;  // nothing of it is seen
+    const bool edge = t0 + TT - 1 > pos_min || t0 + TT > hi || (a.window > 0 && t0 <= pos_max - a.window) || bad;
+#pragma unroll
+    for (int u0 = 0; u0 < U; u0 += UB) {
+      float x[UB][16];
+#pragma unroll
+      for (int u = 0; u < UB; ++u) {
+        if constexpr (kCodes<T>) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            f32x16 sc;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+            for (int k = 4 * g; k < 4 * g + 4; ++k) {
+              const Frag kf = t.k[((u0 + u) * KS + k) * 64 + lane];
+#pragma unroll
+              for (int p = NP - 1; p >= 0; --p) sc = O::mma(kf, qf[k][p], sc);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const f32x4 s4 = *reinterpret_cast<const f32x4*>(&t.ks[g][32 * (u0 + u) + 8 * q + 4 * h]);
+              const f32x4 l4 = *reinterpret_cast<const f32x4*>(&t.kl[g][32 * (u0 + u) + 8 * q + 4 * h]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                x[u][4 * q + e] = __builtin_fmaf(s4[e], sc[4 * q + e], __builtin_fmaf(l4[e], qs[g], x[u][4 * q + e]));
+            }
+          }
+        } else {
+          f32x16 sc;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) sc = O::mma(t.k[((u0 + u) * KS + k) * 64 + lane], qf[k][0], sc);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[u][i] = sc[i];
+        }
+      }
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < UB; ++u)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int tok = t0 + 32 * (u0 + u) + 8 * (i >> 2) + 4 * h + (i & 3);
+            const bool see = tok <= pos && tok < hi && (a.window <= 0 || tok > pos - a.window) &&
+                             !(bad >> (2 * (u0 + u) + (i >> 3)) & 1);
+            x[u][i] = see ? x[u][i] : -__builtin_inff();
+          }
+      }
+      float top = x[0][0] *= rs;
+#pragma unroll
+      for (int u = 0; u < UB; ++u)
+#pragma unroll
+        for (int i = u ? 0 : 1; i < 16; ++i) top = fmaxf(top, x[u][i] *= rs);
+      top = pair_max(top);
+      if (__any(top > m + kSlack)) {
+        const float to = max_of(m, top);
+        const float f = to == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - to);
+        l *= f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) ol[g] *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d) o[d] *= f;
+        m = to;
+      }
+      const float base = m == -__builtin_inff() ? 0.f : m;
+#pragma unroll
+      for (int u = 0; u < UB; ++u)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float p[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            p[e] = __builtin_amdgcn_exp2f(x[u][8 * s + e] - base);
+            l += p[e];
+          }
+          Frag pf[NP];
+          if constexpr (!kCodes<T>) parts_of(p, pf);
+#pragma unroll
+          for (int g = 0; g < G; ++g) {
+            if constexpr (kCodes<T>) {
+              float w[8];
+#pragma unroll
+              for (int q = 0; q < 2; ++q) {
+                const f32x4 s4 = *reinterpret_cast<const f32x4*>(&t.vs[g][32 * (u0 + u) + 16 * s + 8 * q + 4 * h]);
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(&t.vl[g][32 * (u0 + u) + 16 * s + 8 * q + 4 * h]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  w[4 * q + e] = p[4 * q + e] * s4[e];
+                  ol[g] = __builtin_fmaf(p[4 * q + e], l4[e], ol[g]);
+                }
+              }
+              parts_of(w, pf);
+            }
+#pragma unroll
+            for (int d = 2 * g; d < 2 * g + 2; ++d) {
+              const Frag vf = t.v[(d * (TT / 16) + 2 * (u0 + u) + s) * 64 + lane];
+#pragma unroll
+              for (int q = NP - 1; q >= 0; --q) o[d] = O::mma(vf, pf[q], o[d]);
+            }
+          }
+        }
+    }
+  };
+
+  for (int r0 = s0; r0 < s1; r0 += RUN) {
+    const int run = s1 - r0 < RUN ? s1 - r0 : RUN;
+    {
+      const int64_t t = (int64_t)r0 * TT + 16 * lane;
+      const bool used = lane < run * E && t < hi;
+      ids = used ? table[t >> a.shift] : -1;
+      const bool bad = ids < 0 || ids >= a.pages;
+      gone = __ballot(bad);
+      if (bad) ids = 0;  // in bounds, and not seen
+    }
+    Raw raw;
+    load(0, r0, raw);
+    unpack(0, r0, raw, s_tile[0]);
+    load(run > 1 ? 1 : 0, run > 1 ? r0 + 1 : r0, raw);
+    __syncthreads();
+    for (int i = 0; i < run; ++i) {
+      // the next step's tile is written while this one is read, and the loads of the one after are under way
+      if (i + 1 < run) unpack(i + 1, r0 + i + 1, raw, s_tile[(i + 1) & 1]);
+      const int ahead = i + 2 < run ? i + 2 : run - 1;
+      load(ahead, r0 + ahead, raw);
+      compute(i, r0 + i, s_tile[i & 1]);
+      __syncthreads();
+    }
   }
+
+  // a wave has its rows to itself: parts are stored as the registers lie
+  l = pair_sum(l);
+  if constexpr (kCodes<T>)
+#pragma unroll
+    for (int g = 0; g < G; ++g) {
+      const float add = pair_sum(ol[g]);
+#pragma unroll
+      for (int d = 2 * g; d < 2 * g + 2; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] += add;
+    }
+  if (tile.parts > 1) {
+    const int64_t at0 = tile.first * a.Hkv + hk;
+    auto part_at = [&](int part) { return (at0 + (int64_t)part * a.Hkv) * 4 + wave; };  // of waves
+    if (busy) {
+      const int64_t at = part_at(tile.part);
+      f32x4* po = reinterpret_cast<f32x4*>(a.part_o) + at * (DT * 4 * 64) + lane;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          po[(d * 4 + i) * 64] = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
+      if (h == 0) a.part_ml[at * 32 + n] = {m, l};
+    }
+    if (!last_part(a, tile, &s_last)) return;
+    if (!busy) return;
+    float all = -__builtin_inff();
+    for (int c = 0; c < tile.parts; ++c) all = max_of(all, a.part_ml[part_at(c) * 32 + n].x);
+    m = all;
+    const float base = m == -__builtin_inff() ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < tile.parts; ++c) {
+      const int64_t at = part_at(c);
+      const float2 ml = a.part_ml[at * 32 + n];
+      const float f = __builtin_amdgcn_exp2f(ml.x - base);
+      l = __builtin_fmaf(ml.y, f, l);
+      const f32x4* po = reinterpret_cast<const f32x4*>(a.part_o) + at * (DT * 4 * 64) + lane;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 v = po[(d * 4 + i) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][4 * i + e] = __builtin_fmaf(v[e], f, o[d][4 * i + e]);
+        }
+    }
+  }
+  if (!busy || wrow + n >= rows) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* out = static_cast<T*>(a.out) + ((tile.q0 + qi) * ((int64_t)a.Hkv * a.grp) + head) * D;
+#pragma unroll
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {  // words m = 8 q + 4 h + (0..3): 16 values side by side
+      float v[16];
+#pragma unroll
+      for (int w = 0; w < 4; ++w)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * w + j] = o[2 * g + (j >> 1)][8 * (j & 1) + 4 * q + w] * inv;
+      store_values<T, 16>(out + 64 * g + 4 * (8 * q + 4 * h), v);
+    }
 }
 
 // ---- launch -------------------------------------------------------------------------------
+constexpr int kFewRows = 32;
 
 struct Plan {
-  int rt, splits;
-  int64_t tiles;
+  int rt;           // 16-row tiles of k_attend_few, 0: not used
+  bool rows;        // k_attend_rows runs
+  int64_t grid_few, grid_rows;
+  int fill_few, fill_rows;  // blocks that parts fill, 0: no parts
 };
 
-Plan plan_of(int64_t T, int64_t B, int Hkv, int grp, int D, int64_t max_query, int64_t max_context, int64_t window) {
-  Plan p;
-  const int64_t rows = (max_query > 0 && max_query < T ? max_query : T) * grp;
-  p.rt = rows > 16 && D < 256 ? 2 : 1;
-  const int R = 16 * p.rt;
-  p.tiles = T * grp / R + B + 1;
-  // blocks with work: a request's rows fill its tiles but for the last
-  const int64_t real = (cdiv(rows, R) * B < p.tiles ? cdiv(rows, R) * B : p.tiles) * Hkv;
-  int64_t span = max_context;
-  if (window > 0 && span > window + max_query) span = window + max_query;
-  const int64_t most = span / 256;  // two steps a wave at least
-  int64_t s = real > 0 ? cdiv(1024, real) : 1;
-  if (s > most) s = most;
-  p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+// Blocks of one kernel, R rows a tile: a block a tile and head, and with parts `want` more.  Tiles in
+// thousands fill the chip without parts, and the sums over many requests would cost every block more.
+constexpr int kSyncWords = 8192;  // of the workspace's start, one a block
+
+void plan_grid(int64_t T, int64_t B, int Hkv, int grp, int R, int want, int64_t& grid, int& fill) {
+  const int64_t tiles = (T * grp / R + B + 1) * Hkv;
+  fill = tiles <= 4 * want && B < 1024 ? want : 0;
+  if (fill && tiles + fill + Hkv > kSyncWords) fill = 0;
+  grid = tiles + (fill ? fill + Hkv : 0);
+}
+
+Plan plan_of(bool wide, int64_t T, int64_t B, int Hkv, int grp, int64_t max_query) {
+  Plan p{};
+  const int64_t rows = (max_query < T ? max_query : T) * grp;  // of a request
+  // wide: fp32 heads of 256, of which three parts of 32 queries pass the registers
+  p.rt = rows > 16 && !wide ? 2 : 1;
+  p.rows = rows > kFewRows && !wide;
+  if (p.rows && B <= 1) p.rt = 0;
+  if (p.rt) plan_grid(T, B, Hkv, grp, 16 * p.rt, 768, p.grid_few, p.fill_few);
+  if (p.rows) plan_grid(T, B, Hkv, grp, 128, 512, p.grid_rows, p.fill_rows);
   return p;
 }
 
+size_t space_of(const Plan& p, int D) {  // the kernels' parts, which run one after the other
+  const size_t few = p.rt && p.fill_few ? (size_t)p.grid_few * 16 * p.rt : 0;
+  const size_t rows = p.rows && p.fill_rows ? (size_t)p.grid_rows * 128 : 0;
+  const size_t most = few > rows ? few : rows;
+  return most ? (kSyncWords + most * (D + 2)) * sizeof(float) : 0;
+}
+
 template <class T, int D>
-int launch_attend(const AttendArgs& a, const Plan& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.tiles, (unsigned)a.Hkv, (unsigned)p.splits);
-  if (p.rt == 1)
-    hipLaunchKernelGGL((k_kv4_attend<T, D, 1, 4>), grid, dim3(256), 0, s, a);
-  else if constexpr (D < 256)
-    hipLaunchKernelGGL((k_kv4_attend<T, D, 2, 4>), grid, dim3(256), 0, s, a);
-  if (p.splits > 1) {
-    const int64_t rows = a.T * a.Hkv * a.grp;
-    hipLaunchKernelGGL((k_kv4_join<T, D>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a.part_o, a.part_ml, rows,
-                       p.splits, static_cast<T*>(a.out));
+int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
+  constexpr bool wide = kCodes<T> && D == 256;
+  if constexpr (!wide)
+    if (p.rows) {
+      a.part_ml = reinterpret_cast<float2*>(a.part_o + p.grid_rows * 128 * D);
+      a.rows_from = p.rt ? kFewRows + 1 : 0;
+      a.rows_upto = 0x7fffffff;
+      a.blocks = p.fill_rows;
+      a.least = 4;
+      const size_t lds = 2 * sizeof(RowsTile<T, D>);
+      static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attend_rows<T, D>),
+                                                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (allowed != hipSuccess) return hip_check(allowed, "k_attend_rows shared memory");
+      hipLaunchKernelGGL((k_attend_rows<T, D>), dim3((unsigned)p.grid_rows), dim3(256), lds, s, a);
+    }
+  if (p.rt) {
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + p.grid_few * 16 * p.rt * D);
+    a.rows_from = 0;
+    a.rows_upto = p.rows ? kFewRows : 0x7fffffff;
+    a.blocks = p.fill_few;
+    a.least = 8;
+    if (p.rt == 1 || wide)
+      hipLaunchKernelGGL((k_attend_few<T, D, 1, 4>), dim3((unsigned)p.grid_few), dim3(256), 0, s, a);
+    else if constexpr (!wide)
+      hipLaunchKernelGGL((k_attend_few<T, D, 2, 4>), dim3((unsigned)p.grid_few), dim3(256), 0, s, a);
   }
-  return hip_check(hipGetLastError(), "k_kv4_attend launch");
+  return hip_check(hipGetLastError(), "k_attend launch");
 }
 
 template <class T>
@@ -508,8 +1197,8 @@ int check_sizes(int64_t T, int64_t B, int Hkv, int Hq, int D, int64_t page_size)
   if (!kv4_shape_ok(D, page_size))
     return fail(QS_ERR_UNSUPPORTED, "kv4_attend: head size %d, page size %lld", D, (long long)page_size);
   if (T < 0 || B < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv) return fail(QS_ERR_INVALID, "kv4_attend: bad shape");
-  if (B > (1 << 20) || Hkv > 65535 || T * Hq >= (int64_t(1) << 31))
-    return fail(QS_ERR_LIMIT, "kv4_attend: over 2^20 requests, 65535 heads or 2^31 query rows");
+  if (B > (1 << 20) || Hkv > 65535 || T * Hq >= (int64_t(1) << 31) || (T * Hq / 16 + (B + 2) * Hkv) >= (int64_t(1) << 31))
+    return fail(QS_ERR_LIMIT, "kv4_attend: over 2^20 requests, 65535 heads or 2^31 query rows or blocks");
   return QS_OK;
 }
 
@@ -520,9 +1209,11 @@ using namespace qs;
 
 extern "C" size_t qs_kv4_attend_workspace_bytes(int64_t T, int64_t B, int Hkv, int Hq, int D, int64_t page_size,
                                                 int64_t max_query, int64_t max_context, int64_t window) {
+  (void)max_context, (void)window;
   if (check_sizes(T, B, Hkv, Hq, D, page_size) != QS_OK) return 0;
-  const Plan p = plan_of(T, B, Hkv, Hq / Hkv, D, max_query, max_context, window);
-  return p.splits > 1 ? (size_t)p.splits * T * Hq * (D + 2) * sizeof(float) : 0;
+  const size_t narrow = space_of(plan_of(false, T, B, Hkv, Hq / Hkv, max_query), D);
+  const size_t wide = D == 256 ? space_of(plan_of(true, T, B, Hkv, Hq / Hkv, max_query), D) : 0;
+  return narrow > wide ? narrow : wide;
 }
 
 extern "C" int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ldq_h, const uint8_t* cache,
@@ -543,16 +1234,32 @@ extern "C" int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ld
   if (ldq_t % per16 || ldq_h % per16 || !aligned(q, 16) || !aligned(out, 16) || !aligned(cache, 16))
     return fail(QS_ERR_INVALID, "kv4_attend: 16-byte alignment");
   const int grp = Hq / Hkv;
-  const Plan p = plan_of(T, B, Hkv, grp, D, max_query, max_context, window);
-  const int64_t part = (int64_t)p.splits * T * Hq;
-  if (p.splits > 1 && (!workspace || workspace_bytes < (size_t)part * (D + 2) * sizeof(float) || !aligned(workspace, 16)))
+  const Plan p = plan_of(dtype == QS_F32 && D == 256, T, B, Hkv, grp, max_query);
+  const size_t need = space_of(p, D);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QS_ERR_INVALID, "kv4_attend: workspace of qs_kv4_attend_workspace_bytes() bytes, 16-byte aligned");
-  int shift = 0;
-  while ((1 << shift) < page_size) ++shift;
-  AttendArgs a{q, cache, tables, starts, context, out, static_cast<float*>(workspace),
-               reinterpret_cast<float2*>(static_cast<float*>(workspace) + part * D), ldq_t, ldq_h, ld_table, T,
-               (int)pages, (int)page_size, shift, (int)width, Hkv, grp, (int)B,
-               (int)(window < (1 << 30) ? window : 1 << 30), p.splits, scale * 1.44269504088896340736f};
+  AttendArgs a{};
+  a.q = q;
+  a.cache = cache;
+  a.tables = tables;
+  a.starts = starts;
+  a.context = context;
+  a.out = out;
+  a.done = static_cast<int*>(workspace);
+  a.part_o = static_cast<float*>(workspace) + kSyncWords;
+  a.ldq_t = ldq_t;
+  a.ldq_h = ldq_h;
+  a.ld_table = ld_table;
+  a.T = T;
+  a.pages = (int)pages;
+  a.P = (int)page_size;
+  while ((int64_t(1) << a.shift) < page_size) ++a.shift;
+  a.width = (int)width;
+  a.Hkv = Hkv;
+  a.grp = grp;
+  a.B = (int)B;
+  a.window = (int)(window < (1 << 30) ? window : 1 << 30);
+  a.scale_log2 = scale * 1.44269504088896340736f;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == QS_F32) return launch_attend_d<float>(a, p, D, s);
   if (dtype == QS_BF16) return launch_attend_d<__bf16>(a, p, D, s);

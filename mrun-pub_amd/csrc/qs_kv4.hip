@@ -133,9 +133,9 @@ __global__ __launch_bounds__(256) void k_kv4_append(AppendArgs a) {
     const uint32_t c = code4(v, s, lo);
     uint8_t* block = a.cache + (page * a.Hkv + h) * (int64_t)L.bytes();
     if (key) {
-      // nibbles 0 and 1 of four values lie four nibbles apart in their dword; the odd lane's are two up
-      uint32_t w = (c & 0xf) | (c >> 4 & 0xf) << 16 | (c >> 8 & 0xf) << 4 | (c >> 12 & 0xf) << 20;
-      if (m & 1) w <<= 8;
+      // a nibble in each byte: the even lane's low ones, the odd lane's high ones
+      uint32_t w = (c & 0xf) | (c >> 4 & 0xf) << 8 | (c >> 8 & 0xf) << 16 | (c >> 12 & 0xf) << 24;
+      if (m & 1) w <<= 4;
       w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0xB1, 0xf, 0xf, true);  // the neighbour's half
       if (!(m & 1)) *reinterpret_cast<uint32_t*>(block + L.k_dword(row, d)) = w;
       if (m == 0) {
@@ -143,7 +143,9 @@ __global__ __launch_bounds__(256) void k_kv4_append(AppendArgs a) {
         *reinterpret_cast<uint32_t*>(block + L.k_scale(row, g)) = pair;
       }
     } else {
-      *reinterpret_cast<uint16_t*>(block + L.v_word(row, d)) = (uint16_t)c;
+      uint8_t* to = block + L.v_byte(row, d);
+      to[0] = (uint8_t)c;
+      to[2] = (uint8_t)(c >> 8);
       if (m == 0) {
         uint8_t* at = block + L.v_scale(row, g);
         *reinterpret_cast<uint16_t*>(at) = __builtin_bit_cast(uint16_t, s);
@@ -171,15 +173,16 @@ __global__ __launch_bounds__(256) void k_kv4_read(const uint8_t* cache, const in
       const uint8_t* block = cache + (page * Hkv + h) * (int64_t)L.bytes();
       const uint32_t kw = *reinterpret_cast<const uint32_t*>(block + L.k_dword(row, d));
       const uint32_t ks = *reinterpret_cast<const uint32_t*>(block + L.k_scale(row, g));
-      const uint32_t v0 = *reinterpret_cast<const uint16_t*>(block + L.v_word(row, d));
-      const uint32_t v1 = *reinterpret_cast<const uint16_t*>(block + L.v_word(row, d + 4));
+      const uint8_t* v0 = block + L.v_byte(row, d);
+      const uint8_t* v1 = block + L.v_byte(row, d + 4);
+      const uint32_t vw = v0[0] | v0[2] << 8 | v1[0] << 16 | (uint32_t)v1[2] << 24;
       const float vs = f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(block + L.v_scale(row, g)));
       const float vl = f16_bits_to_f32(*reinterpret_cast<const uint16_t*>(block + L.v_scale(row, g) + 8));
       const float sc = f16_bits_to_f32((uint16_t)ks), lo = f16_bits_to_f32((uint16_t)(ks >> 16));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         k[e] = (float)(kw >> Kv4Layout::k_shift(e) & 15) * sc + lo;
-        v[e] = (float)((e < 4 ? v0 : v1) >> Kv4Layout::v_shift(e) & 15) * vs + vl;
+        v[e] = (float)(vw >> (4 * e) & 15) * vs + vl;
       }
     }
     const int64_t at = (t * Hkv + h) * D + d;

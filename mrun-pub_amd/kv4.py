@@ -14,6 +14,7 @@ token's key of 128 values, against 256 in 16 bits.  NaN is stored as 0 and value
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -139,6 +140,11 @@ def read(cache: KV4Cache, layer: int, slots: torch.Tensor, *,
     return k, v
 
 
+@functools.lru_cache(maxsize=512)
+def _attend_space(*sizes: int) -> int:
+    return int(nat.load().qs_kv4_attend_workspace_bytes(*sizes, 0, 0))
+
+
 @nat.inference
 def attend(
     q: torch.Tensor, cache: KV4Cache, layer: int, block_tables: torch.Tensor, query_starts: torch.Tensor,
@@ -158,6 +164,7 @@ def attend(
 
     ``max_query`` and ``max_context`` bound the requests' new tokens and contexts; they choose how
     the work is split, never what is computed, and default to the largest that the shapes allow.
+    ``query_starts`` must not decrease.
     """
     if q.ndim != 3 or q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError("queries must be float32, bfloat16 or float16 [tokens, heads, head_dim]")
@@ -188,13 +195,12 @@ def attend(
         out = torch.empty((T, Hq, D), dtype=q.dtype, device=device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("attention output must be contiguous, 16-byte aligned, of the queries' shape and type")
-    shape = (T, B, cache.kv_heads, Hq, D, cache.page_size, mq, mc, int(window or 0))
-    need = int(nat.load().qs_kv4_attend_workspace_bytes(*shape))
-    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    stream = nat.stream_of(device)
+    need = _attend_space(T, B, cache.kv_heads, Hq, D, cache.page_size, mq)
+    workspace = nat.kept_workspace(device, stream, need) if need else None
     nat.call(
         "qs_kv4_attend", nat.ptr(q), nat.dtype_code(q.dtype), q.stride(0), q.stride(1), base, cache.pages,
         cache.page_size, cache.kv_heads, Hq, D, nat.ptr(block_tables), block_tables.stride(0), width, nat.ptr(starts),
-        nat.ptr(ctx), B, T, mq, mc, s, int(window or 0), nat.ptr(out), nat.ptr(workspace), need,
-        nat.stream_of(device),
+        nat.ptr(ctx), B, T, mq, mc, s, int(window or 0), nat.ptr(out), nat.ptr(workspace), need, stream,
     )
     return out
