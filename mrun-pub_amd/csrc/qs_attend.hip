@@ -18,6 +18,8 @@ namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct AttendArgs {
@@ -366,21 +368,38 @@ __device__ __forceinline__ float load_query(const T* q, float scale_log2, Frag (
   return __builtin_amdgcn_ldexpf(scale_log2, e2);
 }
 
-// This block's part is written: true in the block that is the last of its tile's, which then sees
-// the others' parts.
+// Parts go past this chip part's own cache to where every block sees them (the sc1 bit of a store or
+// load), so that no cache has to be written back or dropped for them.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t shared_at(void* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, bytes, 0x00020000);
+}
+constexpr int kDevice = 16;
+__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t r, int at, f32x4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, kDevice);
+}
+__device__ __forceinline__ f32x4 get4(__amdgpu_buffer_rsrc_t r, int at) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, kDevice));
+}
+__device__ __forceinline__ void put2(__amdgpu_buffer_rsrc_t r, int at, float2 v) {
+  __builtin_amdgcn_raw_buffer_store_b64(u32x2{__float_as_uint(v.x), __float_as_uint(v.y)}, r, at, 0, kDevice);
+}
+__device__ __forceinline__ float2 get2(__amdgpu_buffer_rsrc_t r, int at) {
+  const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, kDevice);
+  return {__uint_as_float(v[0]), __uint_as_float(v[1])};
+}
+
+// This block's part is stored: true in the block that is the last of its tile's.
 __device__ __forceinline__ bool last_part(const AttendArgs& a, const Work& w, int* s_last) {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0): the thread's stores are where all see them
   __syncthreads();
   if (threadIdx.x == 0) {
     int* count = a.done + w.first * a.Hkv + w.hk;
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "agent");
     const int before = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (before == w.parts - 1) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     *s_last = before == w.parts - 1;
   }
   __syncthreads();
-  if (!*s_last) return false;
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-  return true;
+  return *s_last;
 }
 
 // ---- few rows --------------------------------------------------------------------------------
@@ -653,7 +672,9 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
   // join the waves, 16 rows at a time; then, in a tile's last block, its parts the same way
   constexpr int TPR = 64 * NW / 16, C = D / TPR;  // threads a row, values a thread
   const int row_of = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * C;
-  const int64_t tile0 = (tile.first * a.Hkv + hk) * (int64_t)R, tile_step = (int64_t)a.Hkv * R;
+  auto part_rows = [&](int part) {  // row 0 of a part, and what one 16-row tile of it holds
+    return (tile.first * a.Hkv + hk + (int64_t)part * a.Hkv) * R;
+  };
   auto join = [&](int rt, float (&v)[C], float& top, float& all) {
     __syncthreads();
     top = -__builtin_inff();
@@ -702,9 +723,11 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
     if (tile.parts == 1) {
       finish(rt, v, all);
     } else if (tile.row0 + rt * 16 + row_of < rows) {
-      const int64_t at = tile0 + tile.part * tile_step + rt * 16 + row_of;
-      store_values<float, C>(a.part_o + at * D + d0, v);
-      if (d0 == 0) a.part_ml[at] = {top, all};
+      const int64_t at = part_rows(tile.part) + rt * 16;
+      const auto po = shared_at(a.part_o + at * D, 64 * D);
+#pragma unroll
+      for (int c = 0; c < C; c += 4) put4(po, (row_of * D + d0 + c) * 4, f32x4{v[c], v[c + 1], v[c + 2], v[c + 3]});
+      if (d0 == 0) put2(shared_at(a.part_ml + at, 128), row_of * 8, {top, all});
     }
   }
   if (tile.parts == 1 || !last_part(a, tile, &s_last)) return;
@@ -714,25 +737,33 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
     const int live = rows - tile.row0 - rt * 16;  // rows of these 16 that exist
     float2 ml[RN];
     f32x4 acc[RN];
+    int row_at[RN];
 #pragma unroll
     for (int i = 0; i < RN; ++i) {
       ml[i] = {-__builtin_inff(), 0.f};
       acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const int row = i * RI + lane / LR;
+      row_at[i] = row < live ? row : live - 1;
     }
-#pragma unroll 2
-    for (int c = wave; c < tile.parts; c += NW) {
-      const int64_t at = tile0 + c * tile_step + rt * 16 + lane / LR;
+    if (live > 0)
+      for (int c = wave; c < tile.parts; c += NW) {
+        const int64_t at = part_rows(c) + rt * 16;
+        const auto ro = shared_at(a.part_o + at * D, 64 * D), rm = shared_at(a.part_ml + at, 128);
+        float2 pm[RN];
+        f32x4 po[RN];
 #pragma unroll
-      for (int i = 0; i < RN; ++i) {
-        if (i * RI + lane / LR >= live) continue;
-        const float2 pm = a.part_ml[at + i * RI];
-        const f32x4 po = *reinterpret_cast<const f32x4*>(a.part_o + (at + i * RI) * D + (lane % LR) * 4);
-        const float to = max_of(ml[i].x, pm.x), base = to == -__builtin_inff() ? 0.f : to;
-        const float f0 = __builtin_amdgcn_exp2f(ml[i].x - base), f1 = __builtin_amdgcn_exp2f(pm.x - base);
-        ml[i] = {to, ml[i].y * f0 + pm.y * f1};
-        acc[i] = acc[i] * f0 + po * f1;
+        for (int i = 0; i < RN; ++i) {
+          pm[i] = get2(rm, row_at[i] * 8);
+          po[i] = get4(ro, (row_at[i] * D + (lane % LR) * 4) * 4);
+        }
+#pragma unroll
+        for (int i = 0; i < RN; ++i) {
+          const float to = max_of(ml[i].x, pm[i].x), base = to == -__builtin_inff() ? 0.f : to;
+          const float f0 = __builtin_amdgcn_exp2f(ml[i].x - base), f1 = __builtin_amdgcn_exp2f(pm[i].x - base);
+          ml[i] = {to, ml[i].y * f0 + pm[i].y * f1};
+          acc[i] = acc[i] * f0 + po[i] * f1;
+        }
       }
-    }
 #pragma unroll
     for (int i = 0; i < RN; ++i) {
       const int row = i * RI + lane / LR;
@@ -1064,19 +1095,18 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
     auto part_at = [&](int part) { return (at0 + (int64_t)part * a.Hkv) * 4 + wave; };  // of waves
     if (busy) {
       const int64_t at = part_at(tile.part);
-      f32x4* po = reinterpret_cast<f32x4*>(a.part_o) + at * (DT * 4 * 64) + lane;
+      const auto po = shared_at(a.part_o + at * (32 * D), 128 * D);
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          po[(d * 4 + i) * 64] = f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]};
-      if (h == 0) a.part_ml[at * 32 + n] = {m, l};
+          put4(po, ((d * 4 + i) * 64 + lane) * 16, f32x4{o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]});
+      if (h == 0) put2(shared_at(a.part_ml + at * 32, 256), n * 8, {m, l});
     }
     if (!last_part(a, tile, &s_last)) return;
     if (!busy) return;
-    float all = -__builtin_inff();
-    for (int c = 0; c < tile.parts; ++c) all = max_of(all, a.part_ml[part_at(c) * 32 + n].x);
-    m = all;
+    m = -__builtin_inff();
+    for (int c = 0; c < tile.parts; ++c) m = max_of(m, get2(shared_at(a.part_ml + part_at(c) * 32, 256), n * 8).x);
     const float base = m == -__builtin_inff() ? 0.f : m;
     l = 0.f;
 #pragma unroll
@@ -1086,18 +1116,17 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
 #pragma unroll 1
     for (int c = 0; c < tile.parts; ++c) {
       const int64_t at = part_at(c);
-      const float2 ml = a.part_ml[at * 32 + n];
+      const float2 ml = get2(shared_at(a.part_ml + at * 32, 256), n * 8);
+      const auto po = shared_at(a.part_o + at * (32 * D), 128 * D);
+      f32x4 v[DT * 4];
+#pragma unroll
+      for (int i = 0; i < DT * 4; ++i) v[i] = get4(po, (i * 64 + lane) * 16);
       const float f = __builtin_amdgcn_exp2f(ml.x - base);
       l = __builtin_fmaf(ml.y, f, l);
-      const f32x4* po = reinterpret_cast<const f32x4*>(a.part_o) + at * (DT * 4 * 64) + lane;
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int i = 0; i < DT * 4; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const f32x4 v = po[(d * 4 + i) * 64];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[d][4 * i + e] = __builtin_fmaf(v[e], f, o[d][4 * i + e]);
-        }
+        for (int e = 0; e < 4; ++e) o[i / 4][4 * (i % 4) + e] = __builtin_fmaf(v[i][e], f, o[i / 4][4 * (i % 4) + e]);
     }
   }
   if (!busy || wrow + n >= rows) return;
