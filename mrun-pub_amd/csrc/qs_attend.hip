@@ -10,6 +10,8 @@
 // o = sum_t p_t v_t / sum_t p_t with p_t = 2^(x_t - m), x the scores in units of log2 and m their
 // running maximum, one pass over the cache.  Blocks share the requests' tokens out among themselves
 // (pick_work); where several take parts of one tile's tokens, the last of them to finish joins them.
+#include <type_traits>
+
 #include "qs_kv4.h"
 #include "qs_values.h"
 
@@ -34,7 +36,7 @@ struct AttendArgs {
   int* done;        // [block]: parts finished of the tile whose first block it is; 0 between calls
   int64_t ldq_t, ldq_h, ld_table, T;
   int pages, P, shift, width, Hkv, grp, B, window;
-  int blocks, least;        // parts: blocks to fill, steps of a part at least; blocks 0: no parts
+  int blocks, least, whole;  // parts: blocks to fill (0: no parts), steps of a part at least, steps that stay whole
   int rows_from, rows_upto;  // requests of other row counts are the other kernel's
   float scale_log2;
 };
@@ -222,16 +224,33 @@ __device__ __forceinline__ Work pick_tile(const AttendArgs& a, int64_t y, int R)
   return t;
 }
 
-// With parts: a tile whose tokens take W steps is cut into ceil(W / size) parts, size so that the
-// parts of all requests come to about a.blocks blocks.  Every block does the two sums over the
-// requests itself; each thread has B / threads of them.
+// Inclusive sum over the wave, register lane moves only.
+template <int CTRL, int ROW_MASK>
+__device__ __forceinline__ int dpp_from(int v) {
+  return __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan(int v) {
+  v += dpp_from<0x111, 0xf>(v);  // row_shr:1
+  v += dpp_from<0x112, 0xf>(v);
+  v += dpp_from<0x114, 0xf>(v);
+  v += dpp_from<0x118, 0xf>(v);
+  v += dpp_from<0x142, 0xa>(v);  // row_bcast:15
+  v += dpp_from<0x143, 0xc>(v);  // row_bcast:31
+  return v;
+}
+
+// With parts: a tile whose tokens take W steps is cut into ceil(W / size) parts, size so that all
+// requests' tiles and parts come to at most a.blocks blocks, which run at once, if the tiles alone
+// do not pass that.  Every block does the sums over the requests itself: up to 63 requests each of
+// its waves, a lane a request; more with all its threads, and LDS between the waves.
 template <int R, int STEP, int THREADS>
-__device__ __forceinline__ Work pick_part(const AttendArgs& a, int64_t y, int64_t* s_sum, Work* s_work) {
-  const int each = a.B / THREADS + 1;  // of B + 1
-  const int b0 = threadIdx.x * each, b1 = b0 + each < a.B + 1 ? b0 + each : a.B + 1;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_sum, Work* s_work) {
   constexpr int NW = THREADS / 64;
-  int64_t q0;
+  const bool alone = a.B < 64;  // the wave
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int me = alone ? lane : threadIdx.x, each = alone ? 1 : a.B / THREADS + 1;  // of B + 1 requests
+  const int b0 = me * each < a.B + 1 ? me * each : a.B + 1, b1 = b0 + each < a.B + 1 ? b0 + each : a.B + 1;
+  int64_t q0 = 0;
   int n = 0, tiles = 0, steps = 0;
   auto look = [&](int b) {
     q0 = start_of(a, b);
@@ -240,79 +259,106 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int64_t y, int64_
     tiles = mine(a, rows) ? (rows + R - 1) / R : 0;
     const int ctx = context_of(a, b);
     const int64_t reach = (int64_t)a.width << a.shift;
-    int64_t span = ctx < reach ? ctx : reach;
-    if (a.window > 0 && span > (int64_t)a.window + R) span = (int64_t)a.window + R;  // of one tile
-    steps = (int)((span + STEP - 1) / STEP);
+    int span = ctx < reach ? ctx : (int)reach;
+    if (a.window > 0 && span > a.window + R) span = a.window + R;  // of one tile
+    steps = (span + STEP - 1) / STEP;
   };
-  auto block_sum = [&](int64_t v, int64_t& before) {
-    int64_t up = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t o = __shfl_up(up, off, 64);
-      if (lane >= off) up += o;
-    }
-    if (lane == 63) s_sum[wave] = up;
+  auto total_of = [&](float v) {
+    v = wave_sum_dpp(v);
+    if (alone) return v;
     __syncthreads();
-    int64_t all = 0;
-    before = up - v;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      if (w < wave) before += s_sum[w];
-      all += s_sum[w];
-    }
+    if (lane == 0) s_sum[wave] = v;
     __syncthreads();
+    float all = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) all += s_sum[w];
     return all;
   };
-  int64_t sum = 0, before;
+  auto parts_for = [&](float per_step) {
+    if (steps <= a.whole) return 1;
+    return (int)__builtin_ceilf((float)steps * per_step);
+  };
+  float sum = 0.f;
   for (int b = b0; b < b1; ++b) {
     look(b);
-    sum += (int64_t)tiles * steps;
+    sum += (float)tiles * (float)steps;
   }
-  const int64_t total = block_sum(sum, before) * a.Hkv;
-  const int64_t size = total / a.blocks + 1 > a.least ? total / a.blocks + 1 : a.least;
-  auto parts_of_tile = [&]() { return steps > 0 ? (int)((steps + size - 1) / size) : 1; };
-  if (each > 1 || b0 >= b1) {
-    sum = 0;
-    for (int b = b0; b < b1; ++b) {
-      look(b);
-      sum += (int64_t)tiles * parts_of_tile();
-    }
-  } else {
-    sum = (int64_t)tiles * parts_of_tile();
-  }
-  if (threadIdx.x == 0) s_work->any = false;
-  block_sum(sum, before);
-  if (y >= before && y < before + sum) {
+  const float most = (float)a.blocks / (float)a.Hkv;
+  float size = total_of(sum) * 1.00001f / most + 1.f;  // sums of rounded products: never too small
+  if (size < (float)a.least) size = (float)a.least;
+  int count = 0;
+#pragma unroll 1
+  for (int round = 0;; ++round) {
+    const float per_step = 1.f / size;
+    count = 0;
     for (int b = b0; b < b1; ++b) {
       if (each > 1) look(b);
-      const int parts = parts_of_tile();
-      const int64_t here = (int64_t)tiles * parts;
-      if (y < before + here) {
-        const int tile = (int)((y - before) / parts);
-        Work t;
-        t.q0 = q0;
-        t.b = b;
-        t.n = n;
-        t.row0 = (tiles - 1 - tile) * R;
-        t.part = (int)(y - before) - tile * parts;
-        t.parts = parts;
-        t.first = y - t.part;
-        t.hk = 0;
-        t.any = true;
-        *s_work = t;
-        break;
-      }
-      before += here;
+      count += tiles * parts_for(per_step);
     }
+    if (round == 2) break;
+    const float over = total_of((float)count) / most;
+    if (over <= 1.f) break;
+    size *= over < 1.5f ? over : 1.5f;
   }
-  __syncthreads();
-  return *s_work;
+  const float per_step = 1.f / size;
+  int before = wave_scan(count) - count;
+  if (!alone) {
+    __syncthreads();
+    if (lane == 63) s_sum[wave] = __int_as_float(before + count);
+    if (threadIdx.x == 0) s_work->any = false;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) before += __float_as_int(s_sum[w]);
+  }
+  Work t;
+  const bool found = y >= before && y < before + count;
+  if (alone) {
+    const uint64_t who = __ballot(found);
+    if (!who) {
+      t.any = false;
+      return t;
+    }
+    const int from = __builtin_ctzll(who);
+    t.b = from;
+    t.q0 = (int64_t)__builtin_amdgcn_readlane((int)q0, from);  // below 2^31
+    t.n = __builtin_amdgcn_readlane(n, from);
+    before = __builtin_amdgcn_readlane(before, from);
+    tiles = __builtin_amdgcn_readlane(tiles, from);
+    t.parts = __builtin_amdgcn_readlane(parts_for(per_step), from);
+    const int tile = (y - before) / t.parts;
+    t.row0 = (tiles - 1 - tile) * R;
+    t.part = y - before - tile * t.parts;
+    t.any = true;
+  } else {
+    if (found) {
+      for (int b = b0; b < b1; ++b) {
+        if (each > 1) look(b);
+        const int parts = parts_for(per_step);
+        if (y < before + tiles * parts) {
+          const int tile = (y - before) / parts;
+          t.q0 = q0;
+          t.b = b;
+          t.n = n;
+          t.row0 = (tiles - 1 - tile) * R;
+          t.part = y - before - tile * parts;
+          t.parts = parts;
+          t.any = true;
+          *s_work = t;
+          break;
+        }
+        before += tiles * parts;
+      }
+    }
+    __syncthreads();
+    t = *s_work;
+  }
+  t.first = y - t.part;
+  return t;
 }
 
 template <int R, int STEP, int THREADS>
-__device__ __forceinline__ Work pick_work(const AttendArgs& a, int64_t* s_sum, Work* s_work) {
+__device__ __forceinline__ Work pick_work(const AttendArgs& a, float* s_sum, Work* s_work) {
   const unsigned x = blockIdx.x, y = x / (unsigned)a.Hkv;  // heads side by side: each to its own XCD's cache
-  Work t = a.blocks > 0 ? pick_part<R, STEP, THREADS>(a, y, s_sum, s_work) : pick_tile(a, y, R);
+  Work t = a.blocks > 0 ? pick_part<R, STEP, THREADS>(a, (int)y, s_sum, s_work) : pick_tile(a, y, R);
   t.hk = (int)(x - y * (unsigned)a.Hkv);
   t.b = __builtin_amdgcn_readfirstlane(t.b);
   t.n = __builtin_amdgcn_readfirstlane(t.n);
@@ -336,36 +382,59 @@ __device__ __forceinline__ Span span_of(const AttendArgs& a, int b, int pos_min,
   return s;
 }
 
-// The lane's query row as operands: KS pieces of 8 values, `stride` apart from q on; what its scores
-// have to be multiplied by; and for codes, its groups' sums (this lane's part of them).
-template <class T, int KS, int STRIDE, int G, class Frag>
-__device__ __forceinline__ float load_query(const T* q, float scale_log2, Frag (&qf)[KS][kParts<T>], float (&sums)[G]) {
-  float v[KS][8], top = 0.f;
+// The lane's query row: KS pieces of 8 values, STRIDE apart, as operands.
+template <class T, int KS, int STRIDE>
+struct QueryRow {
+  float v[KS][8];
+  __device__ __forceinline__ void load(const T* q) {
 #pragma unroll
-  for (int k = 0; k < KS; ++k) {
-    load_values<T, 8>(q + STRIDE * k, v[k]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) top = max_of(top, __builtin_fabsf(v[k][e]));
+    for (int k = 0; k < KS; ++k) load_values<T, 8>(q + STRIDE * k, v[k]);
   }
-  int e2 = 0;
-  if constexpr (__is_same(T, __bf16)) {
-    top = STRIDE == 32 ? quad_max(top) : pair_max(top);
-    e2 = top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
+  // Returns what the row's scores have to be multiplied by; sums: this lane's part of its groups' sums.
+  template <int G, class Frag>
+  __device__ __forceinline__ float operands(float scale_log2, Frag (&qf)[KS][kParts<T>], float (&sums)[G]) {
+    int e2 = 0;
+    if constexpr (__is_same(T, __bf16)) {
+      float top = 0.f;
 #pragma unroll
-    for (int k = 0; k < KS; ++k)
+      for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[k][e] = __builtin_amdgcn_ldexpf(v[k][e], -e2);
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, __builtin_fabsf(v[k][e]));
+      top = STRIDE == 32 ? quad_max(top) : pair_max(top);
+      e2 = top < __builtin_inff() ? __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+      for (int k = 0; k < KS; ++k)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[k][e] = __builtin_amdgcn_ldexpf(v[k][e], -e2);
+    }
+#pragma unroll
+    for (int g = 0; g < G; ++g) sums[g] = 0.f;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      parts_of(v[k], qf[k]);
+      if constexpr (kCodes<T>)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sums[k * STRIDE / kKv4Group] += v[k][e];
+    }
+    return __builtin_amdgcn_ldexpf(scale_log2, e2);
+  }
+};
+
+// N dwords (1, 2 or a multiple of 4) of a block.
+template <int N>
+__device__ __forceinline__ void fetch(uint32_t* to, __amdgpu_buffer_rsrc_t r, int lane_at, int at) {
+  if constexpr (N == 1) to[0] = __builtin_amdgcn_raw_buffer_load_b32(r, lane_at, at, 0);
+  if constexpr (N == 2) {
+    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(r, lane_at, at, 0);
+    to[0] = v[0];
+    to[1] = v[1];
   }
 #pragma unroll
-  for (int g = 0; g < G; ++g) sums[g] = 0.f;
+  for (int i = 0; i + 3 < N; i += 4) {
+    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(r, lane_at + 4 * i, at, 0);
 #pragma unroll
-  for (int k = 0; k < KS; ++k) {
-    parts_of(v[k], qf[k]);
-    if constexpr (kCodes<T>)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sums[k * STRIDE / kKv4Group] += v[k][e];
+    for (int e = 0; e < 4; ++e) to[i + e] = v[e];
   }
-  return __builtin_amdgcn_ldexpf(scale_log2, e2);
 }
 
 // Parts go past this chip part's own cache to where every block sees them (the sc1 bit of a store or
@@ -403,22 +472,26 @@ __device__ __forceinline__ bool last_part(const AttendArgs& a, const Work& w, in
 }
 
 // ---- few rows --------------------------------------------------------------------------------
-// Whether registers hold two steps' codes besides the queries and results, and the waves a SIMD
-// that they leave room for.
+// Waves a SIMD that the registers leave room for, waves of a block, and blocks that run at once.
 template <class T, int D, int RT>
-constexpr bool kFewAhead = D < 256;
+constexpr bool kFewWide = kCodes<T> ? D * RT >= 256 : D * RT >= 512;
 template <class T, int D, int RT>
-constexpr int kFewWaves = (kCodes<T> ? (RT == 2 ? 1 : 2) : (RT == 2 ? 2 : 3)) + (D == 64 ? 1 : 0) - (D == 256 ? 1 : 0);
+constexpr int kFewWaves = kFewWide<T, D, RT> ? 1 : D * RT * kParts<T> <= 192 ? 4 : 2;
+template <class T, int D, int RT>
+constexpr int kFewBlock = kFewWide<T, D, RT> ? 4 : 8;
+template <class T, int D, int RT>
+constexpr int kFewFill = 256 * 4 * kFewWaves<T, D, RT> / kFewBlock<T, D, RT>;
 
-template <class T, int D, int RT, int NW>
-__global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(AttendArgs a) {
+template <class T, int D, int RT>
+__global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) void k_attend_few(AttendArgs a) {
+  constexpr int NW = kFewBlock<T, D, RT>;
   using O = Ops<T>;
   typedef typename O::Frag Frag;
   constexpr int G = D / kKv4Group, KS = D / 32, R = 16 * RT, W = 2 * G, NP = kParts<T>;
   constexpr int KW = kCodes<T> ? 4 * G : G;  // dwords of key scales: the scores' four tokens, or the operand's own
   __shared__ float s_o[NW][16][D + 4];
   __shared__ float2 s_ml[NW][16];
-  __shared__ int64_t s_sum[NW];
+  __shared__ float s_sum[NW];
   __shared__ Work s_work;
   __shared__ int s_last;
   const int lane = threadIdx.x & 63, n = lane & 15, qq = lane >> 4;
@@ -432,31 +505,85 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
   const Span span = span_of(a, tile.b, pos_min, pos_max);
   const int lo = span.lo, hi = span.hi;
 
-  // queries: the lane's row, values d = 32 i + 8 qq + (0..7)
-  Frag qf[RT][KS][NP];
-  float rs[RT], qs[RT][G];
-  int pos[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    int row = tile.row0 + rt * 16 + n;
-    if (row >= rows) row = rows - 1;
-    const int i = row / a.grp, head = hk * a.grp + row - i * a.grp;
-    pos[rt] = past + i;
-    rs[rt] = load_query<T, KS, 32, G>(static_cast<const T*>(a.q) + (tile.q0 + i) * a.ldq_t + head * a.ldq_h + 8 * qq,
-                                      a.scale_log2, qf[rt], qs[rt]);
-    if constexpr (kCodes<T>)
-#pragma unroll
-      for (int g = 0; g < G; ++g) qs[rt][g] = quad_sum(qs[rt][g]);
-  }
-
   // this block's steps of 32 tokens, of which the wave takes every NW-th
   const int first = lo >> 5, steps = ((hi + 31) >> 5) - first;
   const int s0 = first + (int)((int64_t)steps * tile.part / tile.parts);
   const int s1 = first + (int)((int64_t)steps * (tile.part + 1) / tile.parts);
-
-  const Kv4Layout L(a.P, D);
-  const int64_t block_bytes = L.bytes();
+  const int its = s1 - s0 > wave ? (s1 - s0 - wave + NW - 1) / NW : 0;
   const int* table = a.tables + (int64_t)(tile.b < a.B ? tile.b : 0) * a.ld_table;
+  const Kv4Layout L(a.P, D);
+  const int block_bytes = L.bytes();
+
+  // lane l holds the page of the wave's step l / 2, tokens 16 (l & 1), of a run of 32 steps
+  int ids = -1;
+  uint64_t gone = 0;  // those that are no page
+  auto load_ids = [&](int it0) {
+    const int64_t t = (int64_t)(s0 + wave + NW * (it0 + (lane >> 1))) * 32 + 16 * (lane & 1);
+    ids = it0 + (lane >> 1) < its && t < hi ? table[t >> a.shift] : -1;
+  };
+  load_ids(0);
+
+  struct RawK {
+    uint32_t k[2][KS], s[2][KW];
+  };
+  struct RawV {
+    uint32_t v[2][W], s[2][G][4];
+  };
+  // Codes come through a descriptor of their (page, head) block, so that offsets are one lane
+  // constant and one scalar; no page is a block of no bytes, which reads as zeros.
+  const int k_lane = n * (D / 2) + qq * (KS * 4), ks_lane = (kCodes<T> ? 4 * qq : n) * (G * 4);
+  const int v_lane = qq * (128 * G) + n * (W * 4), vs_lane = qq * (G * 16);
+  auto block_of = [&](int at, int h) {
+    const int id = __builtin_amdgcn_readlane(ids, (2 * at + h) & 63);
+    const bool in = at < 32 && id >= 0 && id < a.pages;
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(a.cache) + ((int64_t)(in ? id : 0) * a.Hkv + hk) * block_bytes, 0, in ? block_bytes : 0, 0x00020000);
+  };
+  auto load_k = [&](int at, int step, RawK& r) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const auto block = block_of(at, h);
+      const int tl = (step * 32 + 16 * h) & (a.P - 1);
+      fetch<KS>(r.k[h], block, k_lane, tl * (D / 2));
+      fetch<KW>(r.s[h], block, ks_lane, L.k_scales() + tl * (G * 4));
+    }
+  };
+  auto load_v = [&](int at, int step, RawV& r) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const auto block = block_of(at, h);
+      const int tl = (step * 32 + 16 * h) & (a.P - 1);
+      fetch<W>(r.v[h], block, v_lane, L.v_codes() + tl * (32 * G));
+      fetch<4 * G>(&r.s[h][0][0], block, vs_lane, L.v_scales() + tl * (G * 4));
+    }
+  };
+
+  // queries: the lane's row, values d = 32 i + 8 qq + (0..7), under way while the pages arrive
+  Frag qf[RT][KS][NP];
+  float rs[RT], qs[RT][G];
+  int pos[RT];
+  QueryRow<T, KS, 32> raw_q[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    int row = tile.row0 + rt * 16 + n;
+    if (row >= rows) row = rows - 1;
+    const int i = (int)((unsigned)row / (unsigned)a.grp), head = hk * a.grp + row - i * a.grp;
+    pos[rt] = past + i;
+    raw_q[rt].load(static_cast<const T*>(a.q) + (tile.q0 + i) * a.ldq_t + head * a.ldq_h + 8 * qq);
+  }
+  RawK rk;
+  RawV rv;
+  if (its > 0) {
+    load_k(0, s0 + wave, rk);
+    load_v(0, s0 + wave, rv);
+  }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    rs[rt] = raw_q[rt].template operands<G>(a.scale_log2, qf[rt], qs[rt]);
+    if constexpr (kCodes<T>)
+#pragma unroll
+      for (int g = 0; g < G; ++g) qs[rt][g] = quad_sum(qs[rt][g]);
+  }
 
   f32x4 o[RT][G][4];
   float m[RT], l[RT], ol[RT][G];  // ol: codes' sum of p lo
@@ -472,30 +599,7 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
     }
   }
 
-  struct Raw {
-    uint32_t k[2][KS], ks[2][KW], v[2][W], vs[2][G][4];
-  };
-  // lane l holds the page of the wave's step l / 2, tokens 16 (l & 1), of a run of 32 steps
-  int ids = -1;
-  uint64_t gone = 0;  // those that are no page
-  auto load = [&](int at, int step, Raw& r) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int t = step * 32 + 16 * h;
-      const int id = __builtin_amdgcn_readlane(ids, 2 * at + h);
-      const uint8_t* block = a.cache + ((int64_t)id * a.Hkv + hk) * block_bytes;
-      const int tl = t & (a.P - 1);
-      const uint8_t* kp = block + (tl + n) * (D / 2) + qq * (KS * 4);
-      const uint8_t* sp = block + L.k_scales() + (tl + (kCodes<T> ? 4 * qq : n)) * (G * 4);
-      const uint8_t* vp = block + L.v_codes() + (tl / 4 + qq) * (32 * W * 4 / 2) + n * (W * 4);
-      const uint8_t* wp = block + L.v_scales() + (tl / 4 + qq) * (G * 16);
-      __builtin_memcpy(r.k[h], __builtin_assume_aligned(kp, KS * 4 < 16 ? KS * 4 : 16), KS * 4);
-      __builtin_memcpy(r.ks[h], __builtin_assume_aligned(sp, KW * 4 < 16 ? KW * 4 : 16), KW * 4);
-      __builtin_memcpy(r.v[h], __builtin_assume_aligned(vp, W * 4 < 16 ? W * 4 : 16), W * 4);
-      __builtin_memcpy(r.vs[h], __builtin_assume_aligned(wp, 16), G * 16);
-    }
-  };
-  auto step_of = [&](int step, int at, Raw& cur) {
+  auto step_of = [&](int step, int at, bool more) {
     const int t0 = step * 32;
     const int bad = (int)(gone >> (2 * at)) & 3;
     const bool edge = t0 + 31 > pos_min || t0 + 32 > hi || t0 < lo || (a.window > 0 && t0 <= pos_max - a.window) || bad;
@@ -509,8 +613,8 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
           const uint32_t keep = (ok && t >= lo && t < hi ? 0xffffu : 0u) | (ok && t + 1 >= lo && t + 1 < hi ? 0xffff0000u : 0u);
 #pragma unroll
           for (int g = 0; g < G; ++g) {
-            cur.vs[h][g][c] &= keep;
-            cur.vs[h][g][2 + c] &= keep;
+            rv.s[h][g][c] &= keep;
+            rv.s[h][g][2 + c] &= keep;
           }
         }
     }
@@ -529,7 +633,7 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
           for (int rt = 0; rt < RT; ++rt) sc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 2 * g; k < 2 * g + 2; ++k) {
-            const Frag kf = O::key(cur.k[h][k], 0);
+            const Frag kf = O::key(rk.k[h][k], 0);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
@@ -537,7 +641,7 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const uint32_t sl = cur.ks[h][r * G + g];
+            const uint32_t sl = rk.s[h][r * G + g];
             const float s = f16_bits_to_f32((uint16_t)sl), z = f16_bits_to_f32((uint16_t)(sl >> 16));
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
@@ -550,7 +654,7 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
         for (int rt = 0; rt < RT; ++rt) sc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const Frag kf = O::key(cur.k[h][k], cur.ks[h][k / 2]);
+          const Frag kf = O::key(rk.k[h][k], rk.s[h][k / 2]);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) sc[rt] = O::mma(kf, qf[rt][k][0], sc[rt]);
         }
@@ -560,6 +664,10 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
           for (int r = 0; r < 4; ++r) x[rt][4 * h + r] = sc[rt][r];
       }
     }
+    // the registers of the keys are free: the next step's are under way through the rest of this one
+    __builtin_amdgcn_sched_barrier(0);
+    load_k(more ? at + 1 : 32, step + NW, rk);
+    __builtin_amdgcn_sched_barrier(0);
     float p[RT][8];
     Frag pf[RT][NP];
 #pragma unroll
@@ -601,9 +709,9 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
       uint32_t u[4], s[4], z[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {  // token pairs (0, 1), (2, 3) of both tiles' units
-        u[i] = cur.v[i >> 1][2 * g + (i & 1)];
-        s[i] = cur.vs[i >> 1][g][i & 1];
-        z[i] = cur.vs[i >> 1][g][2 + (i & 1)];
+        u[i] = rv.v[i >> 1][2 * g + (i & 1)];
+        s[i] = rv.s[i >> 1][g][i & 1];
+        z[i] = rv.s[i >> 1][g][2 + (i & 1)];
       }
       if constexpr (kCodes<T>) {
 #pragma unroll
@@ -629,44 +737,21 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
       product(O::template val<2>(u, s, z), 2);
       product(O::template val<3>(u, s, z), 3);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    load_v(more ? at + 1 : 32, step + NW, rv);
+    __builtin_amdgcn_sched_barrier(0);
   };
 
-  const int its = s1 - s0 > wave ? (s1 - s0 - wave + NW - 1) / NW : 0;
   for (int it0 = 0; it0 < its; it0 += 32) {
     const int run = its - it0 < 32 ? its - it0 : 32;
     const int base = s0 + wave + NW * it0;
-    {
-      const int64_t t = (int64_t)(base + NW * (lane >> 1)) * 32 + 16 * (lane & 1);
-      ids = (lane >> 1) < run && t < hi ? table[t >> a.shift] : -1;
-      const bool bad = ids < 0 || ids >= a.pages;
-      gone = __ballot(bad);
-      if (bad) ids = 0;  // in bounds, and not seen
+    if (it0 > 0) {
+      load_ids(it0);
+      load_k(0, base, rk);
+      load_v(0, base, rv);
     }
-    Raw ra;
-    auto fetch = [&](int i, Raw& r) {
-      i = i < run ? i : run - 1;
-      load(i, base + NW * i, r);
-    };
-    fetch(0, ra);
-    if constexpr (kFewAhead<T, D, RT>) {
-      // the next steps' loads are under way while one is computed; past the end the last is read again
-      Raw rb;
-      fetch(1, rb);
-      for (int i = 0;; i += 2) {
-        step_of(base + NW * i, i, ra);
-        if (i + 1 >= run) break;
-        fetch(i + 2, ra);
-        step_of(base + NW * (i + 1), i + 1, rb);
-        if (i + 2 >= run) break;
-        fetch(i + 3, rb);
-      }
-    } else {
-      for (int i = 0;; ++i) {
-        step_of(base + NW * i, i, ra);
-        if (i + 1 >= run) break;
-        fetch(i + 1, ra);
-      }
-    }
+    gone = __ballot(ids < 0 || ids >= a.pages);
+    for (int i = 0; i < run; ++i) step_of(base + NW * i, i, i + 1 < run);
   }
 
   // join the waves, 16 rows at a time; then, in a tile's last block, its parts the same way
@@ -726,7 +811,8 @@ __global__ __launch_bounds__(64 * NW, (kFewWaves<T, D, RT>)) void k_attend_few(A
       const int64_t at = part_rows(tile.part) + rt * 16;
       const auto po = shared_at(a.part_o + at * D, 64 * D);
 #pragma unroll
-      for (int c = 0; c < C; c += 4) put4(po, (row_of * D + d0 + c) * 4, f32x4{v[c], v[c + 1], v[c + 2], v[c + 3]});
+      for (int c = 0; c + 3 < C; c += 4) put4(po, (row_of * D + d0 + c) * 4, f32x4{v[c], v[c + 1], v[c + 2], v[c + 3]});
+      if constexpr (C == 2) put2(po, (row_of * D + d0) * 4, {v[0], v[1]});
       if (d0 == 0) put2(shared_at(a.part_ml + at, 128), row_of * 8, {top, all});
     }
   }
@@ -804,7 +890,7 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
   constexpr int KG = D == 64 ? 1 : 2;         // groups that a thread's dwords of keys belong to
   extern __shared__ __attribute__((aligned(16))) char s_mem[];
   Tile* s_tile = reinterpret_cast<Tile*>(s_mem);  // two
-  __shared__ int64_t s_sum[4];
+  __shared__ float s_sum[4];
   __shared__ Work s_work;
   __shared__ int s_last;
   const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
@@ -827,8 +913,9 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
   const int pos = past + qi;
   Frag qf[KS][NP];
   float qs[G];
-  const float rs = load_query<T, KS, 16, G>(static_cast<const T*>(a.q) + (tile.q0 + qi) * a.ldq_t + head * a.ldq_h + 8 * h,
-                                            a.scale_log2, qf, qs);
+  QueryRow<T, KS, 16> raw_q;
+  raw_q.load(static_cast<const T*>(a.q) + (tile.q0 + qi) * a.ldq_t + head * a.ldq_h + 8 * h);
+  const float rs = raw_q.template operands<G>(a.scale_log2, qf, qs);
   if constexpr (kCodes<T>)
 #pragma unroll
     for (int g = 0; g < G; ++g) qs[g] = pair_sum(qs[g]);
@@ -1158,6 +1245,7 @@ struct Plan {
 // Blocks of one kernel, R rows a tile: a block a tile and head, and with parts `want` more.  Tiles in
 // thousands fill the chip without parts, and the sums over many requests would cost every block more.
 constexpr int kSyncWords = 8192;  // of the workspace's start, one a block
+constexpr int kFill = 512;        // blocks that parts fill, at most
 
 void plan_grid(int64_t T, int64_t B, int Hkv, int grp, int R, int want, int64_t& grid, int& fill) {
   const int64_t tiles = (T * grp / R + B + 1) * Hkv;
@@ -1173,8 +1261,8 @@ Plan plan_of(bool wide, int64_t T, int64_t B, int Hkv, int grp, int64_t max_quer
   p.rt = rows > 16 && !wide ? 2 : 1;
   p.rows = rows > kFewRows && !wide;
   if (p.rows && B <= 1) p.rt = 0;
-  if (p.rt) plan_grid(T, B, Hkv, grp, 16 * p.rt, 768, p.grid_few, p.fill_few);
-  if (p.rows) plan_grid(T, B, Hkv, grp, 128, 512, p.grid_rows, p.fill_rows);
+  if (p.rt) plan_grid(T, B, Hkv, grp, 16 * p.rt, kFill, p.grid_few, p.fill_few);
+  if (p.rows) plan_grid(T, B, Hkv, grp, 128, kFill, p.grid_rows, p.fill_rows);
   return p;
 }
 
@@ -1195,6 +1283,7 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
       a.rows_upto = 0x7fffffff;
       a.blocks = p.fill_rows;
       a.least = 4;
+      a.whole = 8;
       const size_t lds = 2 * sizeof(RowsTile<T, D>);
       static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attend_rows<T, D>),
                                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -1205,12 +1294,18 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
     a.part_ml = reinterpret_cast<float2*>(a.part_o + p.grid_few * 16 * p.rt * D);
     a.rows_from = 0;
     a.rows_upto = p.rows ? kFewRows : 0x7fffffff;
-    a.blocks = p.fill_few;
-    a.least = 8;
-    if (p.rt == 1 || wide)
-      hipLaunchKernelGGL((k_attend_few<T, D, 1, 4>), dim3((unsigned)p.grid_few), dim3(256), 0, s, a);
+    a.least = 32;
+    a.whole = 64;
+    auto go = [&](auto rt) {
+      constexpr int RT = decltype(rt)::value;
+      static_assert(kFewFill<T, D, RT> <= kFill);
+      a.blocks = p.fill_few ? kFewFill<T, D, RT> : 0;
+      hipLaunchKernelGGL((k_attend_few<T, D, RT>), dim3((unsigned)p.grid_few), dim3(64 * kFewBlock<T, D, RT>), 0, s, a);
+    };
+    if (p.rt == 1)
+      go(std::integral_constant<int, 1>{});
     else if constexpr (!wide)
-      hipLaunchKernelGGL((k_attend_few<T, D, 2, 4>), dim3((unsigned)p.grid_few), dim3(256), 0, s, a);
+      go(std::integral_constant<int, 2>{});
   }
   return hip_check(hipGetLastError(), "k_attend launch");
 }
