@@ -34,8 +34,9 @@ struct AttendArgs {
   float* part_o;    // [block][rows of a tile * D]
   float2* part_ml;  // [block][rows of a tile]
   int* done;        // [block]: parts finished of the tile whose first block it is; 0 between calls
-  int64_t ldq_t, ldq_h, ld_table, T;
-  int pages, P, shift, width, Hkv, grp, B, window;
+  int64_t ldq_t, ldq_h, ld_table;
+  int pages, P, shift, Hkv, grp, T, B, window;
+  int reach;                // tokens that a table row has room for, 2^30 at most
   int blocks, least, whole;  // parts: blocks to fill (0: no parts), steps of a part at least, steps that stay whole
   int rows_from, rows_upto;  // requests of other row counts are the other kernel's
   float scale_log2;
@@ -258,8 +259,7 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
     const int rows = n * a.grp;
     tiles = mine(a, rows) ? (rows + R - 1) / R : 0;
     const int ctx = context_of(a, b);
-    const int64_t reach = (int64_t)a.width << a.shift;
-    int span = ctx < reach ? ctx : (int)reach;
+    int span = ctx < a.reach ? ctx : a.reach;
     if (a.window > 0 && span > a.window + R) span = a.window + R;  // of one tile
     steps = (span + STEP - 1) / STEP;
   };
@@ -284,21 +284,23 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
     sum += (float)tiles * (float)steps;
   }
   const float most = (float)a.blocks / (float)a.Hkv;
-  float size = total_of(sum) * 1.00001f / most + 1.f;  // sums of rounded products: never too small
+  const float total = total_of(sum);
+  float size = total * 1.00001f / most + 1.f;  // sums of rounded products: never too small
   if (size < (float)a.least) size = (float)a.least;
   int count = 0;
 #pragma unroll 1
   for (int round = 0;; ++round) {
-    const float per_step = 1.f / size;
     count = 0;
     for (int b = b0; b < b1; ++b) {
       if (each > 1) look(b);
-      count += tiles * parts_for(per_step);
+      count += tiles * parts_for(1.f / size);
     }
-    if (round == 2) break;
-    const float over = total_of((float)count) / most;
-    if (over <= 1.f) break;
-    size *= over < 1.5f ? over : 1.5f;
+    if (round == 3) break;
+    const float all = total_of((float)count);
+    if (all <= most) break;
+    // what rounding up adds to total / size parts changes little with the size
+    const float room = most - (all - total / size);
+    size = room > 0.5f * total / size ? total * 1.001f / room : 2.f * size;
   }
   const float per_step = 1.f / size;
   int before = wave_scan(count) - count;
@@ -375,8 +377,7 @@ struct Span {
 __device__ __forceinline__ Span span_of(const AttendArgs& a, int b, int pos_min, int pos_max) {
   Span s;
   s.hi = pos_max + 1;
-  const int64_t reach = (int64_t)a.width << a.shift;
-  if (s.hi > reach) s.hi = (int)reach;
+  if (s.hi > a.reach) s.hi = a.reach;
   s.lo = a.window > 0 && pos_min - a.window + 1 > 0 ? pos_min - a.window + 1 : 0;
   if (b >= a.B || s.hi < s.lo) s.hi = s.lo;
   return s;
@@ -483,7 +484,10 @@ template <class T, int D, int RT>
 constexpr int kFewFill = 256 * 4 * kFewWaves<T, D, RT> / kFewBlock<T, D, RT>;
 
 template <class T, int D, int RT>
-__global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) void k_attend_few(AttendArgs a) {
+__global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) void k_attend_few(
+    const int* starts, const int* context, int tokens, int requests, int Hkv, int grp, int reach, int window, int blocks, AttendArgs a) {
+  a.starts = starts, a.context = context, a.T = tokens, a.B = requests, a.Hkv = Hkv, a.grp = grp, a.reach = reach;
+  a.window = window, a.blocks = blocks;
   constexpr int NW = kFewBlock<T, D, RT>;
   using O = Ops<T>;
   typedef typename O::Frag Frag;
@@ -817,44 +821,54 @@ __global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) 
     }
   }
   if (tile.parts == 1 || !last_part(a, tile, &s_last)) return;
-  constexpr int RI = 256 / D, RN = 16 / RI, LR = 64 / RI;  // rows a pass of four values a lane, passes, lanes a row
+  // a wave takes every NW-th part, four of them and two sets of RI rows at a time
+  constexpr int RI = 256 / D, LR = 64 / RI;  // rows of a set, lanes a row
 #pragma unroll 1
   for (int rt = 0; rt < RT; ++rt) {
-    const int live = rows - tile.row0 - rt * 16;  // rows of these 16 that exist
-    float2 ml[RN];
-    f32x4 acc[RN];
-    int row_at[RN];
+    const int live = rows - tile.row0 - rt * 16 < 16 ? rows - tile.row0 - rt * 16 : 16;  // rows that exist
+#pragma unroll 1
+    for (int i0 = 0; i0 < live; i0 += 2 * RI) {
+      float2 ml[2];
+      f32x4 acc[2];
+      int row[2];
 #pragma unroll
-    for (int i = 0; i < RN; ++i) {
-      ml[i] = {-__builtin_inff(), 0.f};
-      acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int row = i * RI + lane / LR;
-      row_at[i] = row < live ? row : live - 1;
-    }
-    if (live > 0)
-      for (int c = wave; c < tile.parts; c += NW) {
-        const int64_t at = part_rows(c) + rt * 16;
-        const auto ro = shared_at(a.part_o + at * D, 64 * D), rm = shared_at(a.part_ml + at, 128);
-        float2 pm[RN];
-        f32x4 po[RN];
+      for (int i = 0; i < 2; ++i) {
+        ml[i] = {-__builtin_inff(), 0.f};
+        acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        row[i] = i0 + i * RI + lane / LR;
+      }
+      for (int c0 = wave; c0 < tile.parts; c0 += 4 * NW) {
+        float2 pm[4][2];
+        f32x4 po[4][2];
 #pragma unroll
-        for (int i = 0; i < RN; ++i) {
-          pm[i] = get2(rm, row_at[i] * 8);
-          po[i] = get4(ro, (row_at[i] * D + (lane % LR) * 4) * 4);
+        for (int c = 0; c < 4; ++c) {
+          const bool in = c0 + c * NW < tile.parts;
+          const int64_t at = part_rows(in ? c0 + c * NW : c0) + rt * 16;
+          const auto ro = shared_at(a.part_o + at * D, in ? 4 * D * live : 0);
+          const auto rm = shared_at(a.part_ml + at, in ? 8 * live : 0);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            pm[c][i] = get2(rm, row[i] * 8);
+            po[c][i] = get4(ro, (row[i] * D + (lane % LR) * 4) * 4);
+          }
         }
 #pragma unroll
-        for (int i = 0; i < RN; ++i) {
-          const float to = max_of(ml[i].x, pm[i].x), base = to == -__builtin_inff() ? 0.f : to;
-          const float f0 = __builtin_amdgcn_exp2f(ml[i].x - base), f1 = __builtin_amdgcn_exp2f(pm[i].x - base);
-          ml[i] = {to, ml[i].y * f0 + pm[i].y * f1};
-          acc[i] = acc[i] * f0 + po[i] * f1;
-        }
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            if (c0 + c * NW >= tile.parts) continue;
+            const float to = max_of(ml[i].x, pm[c][i].x), base = to == -__builtin_inff() ? 0.f : to;
+            const float f0 = __builtin_amdgcn_exp2f(ml[i].x - base), f1 = __builtin_amdgcn_exp2f(pm[c][i].x - base);
+            ml[i] = {to, ml[i].y * f0 + pm[c][i].y * f1};
+            acc[i] = acc[i] * f0 + po[c][i] * f1;
+          }
       }
 #pragma unroll
-    for (int i = 0; i < RN; ++i) {
-      const int row = i * RI + lane / LR;
-      if (lane % LR == 0) s_ml[wave][row] = ml[i];
-      *reinterpret_cast<f32x4*>(&s_o[wave][row][(lane % LR) * 4]) = acc[i];
+      for (int i = 0; i < 2; ++i) {
+        if (row[i] >= 16) continue;
+        if (lane % LR == 0) s_ml[wave][row[i]] = ml[i];
+        *reinterpret_cast<f32x4*>(&s_o[wave][row[i]][(lane % LR) * 4]) = acc[i];
+      }
     }
     float v[C], top, all;
     join(rt, v, top, all);
@@ -880,7 +894,10 @@ struct RowsTile {
 };
 
 template <class T, int D>
-__global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) void k_attend_rows(AttendArgs a) {
+__global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) void k_attend_rows(
+    const int* starts, const int* context, int tokens, int requests, int Hkv, int grp, int reach, int window, int blocks, AttendArgs a) {
+  a.starts = starts, a.context = context, a.T = tokens, a.B = requests, a.Hkv = Hkv, a.grp = grp, a.reach = reach;
+  a.window = window, a.blocks = blocks;
   using O = Ops<T>;
   typedef typename O::Frag Frag;
   typedef RowsTile<T, D> Tile;
@@ -1288,7 +1305,8 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
       static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attend_rows<T, D>),
                                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
       if (allowed != hipSuccess) return hip_check(allowed, "k_attend_rows shared memory");
-      hipLaunchKernelGGL((k_attend_rows<T, D>), dim3((unsigned)p.grid_rows), dim3(256), lds, s, a);
+      hipLaunchKernelGGL((k_attend_rows<T, D>), dim3((unsigned)p.grid_rows), dim3(256), lds, s, a.starts, a.context, a.T,
+                       a.B, a.Hkv, a.grp, a.reach, a.window, a.blocks, a);
     }
   if (p.rt) {
     a.part_ml = reinterpret_cast<float2*>(a.part_o + p.grid_few * 16 * p.rt * D);
@@ -1300,7 +1318,8 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
       constexpr int RT = decltype(rt)::value;
       static_assert(kFewFill<T, D, RT> <= kFill);
       a.blocks = p.fill_few ? kFewFill<T, D, RT> : 0;
-      hipLaunchKernelGGL((k_attend_few<T, D, RT>), dim3((unsigned)p.grid_few), dim3(64 * kFewBlock<T, D, RT>), 0, s, a);
+      hipLaunchKernelGGL((k_attend_few<T, D, RT>), dim3((unsigned)p.grid_few), dim3(64 * kFewBlock<T, D, RT>), 0, s,
+                         a.starts, a.context, a.T, a.B, a.Hkv, a.grp, a.reach, a.window, a.blocks, a);
     };
     if (p.rt == 1)
       go(std::integral_constant<int, 1>{});
@@ -1374,11 +1393,11 @@ extern "C" int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ld
   a.ldq_t = ldq_t;
   a.ldq_h = ldq_h;
   a.ld_table = ld_table;
-  a.T = T;
+  a.T = (int)T;
   a.pages = (int)pages;
   a.P = (int)page_size;
   while ((int64_t(1) << a.shift) < page_size) ++a.shift;
-  a.width = (int)width;
+  a.reach = (int)(width << a.shift < (1 << 30) ? width << a.shift : 1 << 30);
   a.Hkv = Hkv;
   a.grp = grp;
   a.B = (int)B;
