@@ -473,18 +473,19 @@ __device__ __forceinline__ bool last_part(const AttendArgs& a, const Work& w, in
 }
 
 // ---- few rows --------------------------------------------------------------------------------
-// Waves a SIMD that the registers leave room for, waves of a block, and blocks that run at once.
+// AHEAD: registers hold the next step's codes too, which hides a load's time where few waves run;
+// the other form leaves room for twice the waves where their number does that.
 template <class T, int D, int RT>
 constexpr bool kFewWide = kCodes<T> ? D * RT >= 256 : D * RT >= 512;
+template <class T, int D, int RT, bool AHEAD>
+constexpr int kFewWaves = kFewWide<T, D, RT> ? 1 : !AHEAD && D * RT * kParts<T> <= 192 ? 4 : 2;  // a SIMD
 template <class T, int D, int RT>
-constexpr int kFewWaves = kFewWide<T, D, RT> ? 1 : D * RT * kParts<T> <= 192 ? 4 : 2;
-template <class T, int D, int RT>
-constexpr int kFewBlock = kFewWide<T, D, RT> ? 4 : 8;
-template <class T, int D, int RT>
-constexpr int kFewFill = 256 * 4 * kFewWaves<T, D, RT> / kFewBlock<T, D, RT>;
+constexpr int kFewBlock = kFewWide<T, D, RT> ? 4 : 8;  // waves of a block
+template <class T, int D, int RT, bool AHEAD>
+constexpr int kFewFill = 1024 * kFewWaves<T, D, RT, AHEAD> / kFewBlock<T, D, RT>;  // blocks that run at once
 
-template <class T, int D, int RT>
-__global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) void k_attend_few(
+template <class T, int D, int RT, bool AHEAD>
+__global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT, AHEAD>)) void k_attend_few(
     const int* starts, const int* context, int tokens, int requests, int Hkv, int grp, int reach, int window, int blocks, AttendArgs a) {
   a.starts = starts, a.context = context, a.T = tokens, a.B = requests, a.Hkv = Hkv, a.grp = grp, a.reach = reach;
   a.window = window, a.blocks = blocks;
@@ -575,11 +576,11 @@ __global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) 
     pos[rt] = past + i;
     raw_q[rt].load(static_cast<const T*>(a.q) + (tile.q0 + i) * a.ldq_t + head * a.ldq_h + 8 * qq);
   }
-  RawK rk;
-  RawV rv;
+  RawK rk[AHEAD ? 2 : 1];
+  RawV rv[AHEAD ? 2 : 1];
   if (its > 0) {
-    load_k(0, s0 + wave, rk);
-    load_v(0, s0 + wave, rv);
+    load_k(0, s0 + wave, rk[0]);
+    load_v(0, s0 + wave, rv[0]);
   }
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -603,7 +604,13 @@ __global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) 
     }
   }
 
-  auto step_of = [&](int step, int at, bool more) {
+  auto step_of = [&](int step, int at, bool more, RawK& rk, RawV& rv, RawK& next_k, RawV& next_v) {
+    const int ahead = more ? at + 1 : 32;  // past the run's end: no bytes
+    if constexpr (AHEAD) {
+      load_k(ahead, step + NW, next_k);
+      load_v(ahead, step + NW, next_v);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     const int t0 = step * 32;
     const int bad = (int)(gone >> (2 * at)) & 3;
     const bool edge = t0 + 31 > pos_min || t0 + 32 > hi || t0 < lo || (a.window > 0 && t0 <= pos_max - a.window) || bad;
@@ -668,10 +675,11 @@ __global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) 
           for (int r = 0; r < 4; ++r) x[rt][4 * h + r] = sc[rt][r];
       }
     }
-    // the registers of the keys are free: the next step's are under way through the rest of this one
-    __builtin_amdgcn_sched_barrier(0);
-    load_k(more ? at + 1 : 32, step + NW, rk);
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!AHEAD) {  // the registers of the keys are free: the next step's are under way from here
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(ahead, step + NW, next_k);
+      __builtin_amdgcn_sched_barrier(0);
+    }
     float p[RT][8];
     Frag pf[RT][NP];
 #pragma unroll
@@ -741,9 +749,11 @@ __global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) 
       product(O::template val<2>(u, s, z), 2);
       product(O::template val<3>(u, s, z), 3);
     }
-    __builtin_amdgcn_sched_barrier(0);
-    load_v(more ? at + 1 : 32, step + NW, rv);
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!AHEAD) {
+      __builtin_amdgcn_sched_barrier(0);
+      load_v(ahead, step + NW, next_v);
+      __builtin_amdgcn_sched_barrier(0);
+    }
   };
 
   for (int it0 = 0; it0 < its; it0 += 32) {
@@ -751,55 +761,40 @@ __global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) 
     const int base = s0 + wave + NW * it0;
     if (it0 > 0) {
       load_ids(it0);
-      load_k(0, base, rk);
-      load_v(0, base, rv);
+      load_k(0, base, rk[0]);
+      load_v(0, base, rv[0]);
     }
     gone = __ballot(ids < 0 || ids >= a.pages);
-    for (int i = 0; i < run; ++i) step_of(base + NW * i, i, i + 1 < run);
+    if constexpr (AHEAD) {
+      for (int i = 0;; i += 2) {
+        step_of(base + NW * i, i, i + 1 < run, rk[0], rv[0], rk[1], rv[1]);
+        if (i + 1 >= run) break;
+        step_of(base + NW * (i + 1), i + 1, i + 2 < run, rk[1], rv[1], rk[0], rv[0]);
+        if (i + 2 >= run) break;
+      }
+    } else {
+      for (int i = 0; i < run; ++i) step_of(base + NW * i, i, i + 1 < run, rk[0], rv[0], rk[0], rv[0]);
+    }
   }
 
-  // join the waves, 16 rows at a time; then, in a tile's last block, its parts the same way
+  // join the waves, 16 rows at a time
   constexpr int TPR = 64 * NW / 16, C = D / TPR;  // threads a row, values a thread
-  const int row_of = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * C;
-  auto part_rows = [&](int part) {  // row 0 of a part, and what one 16-row tile of it holds
-    return (tile.first * a.Hkv + hk + (int64_t)part * a.Hkv) * R;
-  };
-  auto join = [&](int rt, float (&v)[C], float& top, float& all) {
-    __syncthreads();
-    top = -__builtin_inff();
-#pragma unroll
-    for (int w = 0; w < NW; ++w) top = max_of(top, s_ml[w][row_of].x);
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    all = 0.f;
-#pragma unroll
-    for (int c = 0; c < C; ++c) v[c] = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float2 ml = s_ml[w][row_of];
-      const float f = __builtin_amdgcn_exp2f(ml.x - base);
-      all = __builtin_fmaf(ml.y, f, all);
-#pragma unroll
-      for (int c = 0; c < C; ++c) v[c] = __builtin_fmaf(s_o[w][row_of][d0 + c], f, v[c]);
-    }
-    __syncthreads();
-  };
-  auto finish = [&](int rt, float (&v)[C], float all) {
-    const int row = tile.row0 + rt * 16 + row_of;
-    if (row >= rows) return;
-    const int i = row / a.grp;
-    const int64_t at = (tile.q0 + i) * ((int64_t)a.Hkv * a.grp) + hk * a.grp + row - i * a.grp;
-    const float inv = all == 0.f ? 0.f : 1.f / all;
-#pragma unroll
-    for (int c = 0; c < C; ++c) v[c] *= inv;
-    store_values<T, C>(static_cast<T*>(a.out) + at * D + d0, v);
+  const int live = rows - tile.row0 < R ? rows - tile.row0 : R;  // rows that exist
+  auto part_row = [&](int part) { return (tile.first * a.Hkv + hk + (int64_t)part * a.Hkv) * R; };  // the part's row 0
+  auto out_at = [&](int r) {
+    const int row = tile.row0 + r, i = (int)((unsigned)row / (unsigned)a.grp);
+    return static_cast<T*>(a.out) + ((tile.q0 + i) * ((int64_t)a.Hkv * a.grp) + hk * a.grp + row - i * a.grp) * D;
   };
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
+    if (rt * 16 >= live) break;
     const float sum = quad_sum(l[rt]);
+    if (rt) __syncthreads();
     if (qq == 0) s_ml[wave][n] = {m[rt], sum};
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const float add = kCodes<T> ? quad_sum(ol[rt][g]) : 0.f;
+      if (rt * 16 + n >= live) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         f32x4 w = {o[rt][g][0][r], o[rt][g][1][r], o[rt][g][2][r], o[rt][g][3][r]};
@@ -807,72 +802,103 @@ __global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT>)) 
         *reinterpret_cast<f32x4*>(&s_o[wave][n][64 * g + 16 * qq + 4 * r]) = w;
       }
     }
-    float v[C], top, all;
-    join(rt, v, top, all);
-    if (tile.parts == 1) {
-      finish(rt, v, all);
-    } else if (tile.row0 + rt * 16 + row_of < rows) {
-      const int64_t at = part_rows(tile.part) + rt * 16;
-      const auto po = shared_at(a.part_o + at * D, 64 * D);
+    __syncthreads();
+    const int r16 = threadIdx.x / TPR, d0 = (threadIdx.x % TPR) * C, r = rt * 16 + r16;
+    if (r >= live) continue;
+    float top = -__builtin_inff(), all = 0.f, v[C] = {};
 #pragma unroll
-      for (int c = 0; c + 3 < C; c += 4) put4(po, (row_of * D + d0 + c) * 4, f32x4{v[c], v[c + 1], v[c + 2], v[c + 3]});
-      if constexpr (C == 2) put2(po, (row_of * D + d0) * 4, {v[0], v[1]});
-      if (d0 == 0) put2(shared_at(a.part_ml + at, 128), row_of * 8, {top, all});
+    for (int w = 0; w < NW; ++w) top = max_of(top, s_ml[w][r16].x);
+    const float base = top == -__builtin_inff() ? 0.f : top;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const float2 ml = s_ml[w][r16];
+      const float f = __builtin_amdgcn_exp2f(ml.x - base);
+      all = __builtin_fmaf(ml.y, f, all);
+#pragma unroll
+      for (int c = 0; c < C; ++c) v[c] = __builtin_fmaf(s_o[w][r16][d0 + c], f, v[c]);
+    }
+    if (tile.parts == 1) {
+      const float inv = all == 0.f ? 0.f : 1.f / all;
+#pragma unroll
+      for (int c = 0; c < C; ++c) v[c] *= inv;
+      store_values<T, C>(out_at(r) + d0, v);
+    } else {
+      const int64_t at = part_row(tile.part);
+      const auto po = shared_at(a.part_o + at * D, 4 * R * D);
+#pragma unroll
+      for (int c = 0; c + 3 < C; c += 4) put4(po, (r * D + d0 + c) * 4, f32x4{v[c], v[c + 1], v[c + 2], v[c + 3]});
+      if constexpr (C == 2) put2(po, (r * D + d0) * 4, {v[0], v[1]});
+      if (d0 == 0) put2(shared_at(a.part_ml + at, 8 * R), r * 8, {top, all});
     }
   }
   if (tile.parts == 1 || !last_part(a, tile, &s_last)) return;
-  // a wave takes every NW-th part, four of them and two sets of RI rows at a time
-  constexpr int RI = 256 / D, LR = 64 / RI;  // rows of a set, lanes a row
-#pragma unroll 1
-  for (int rt = 0; rt < RT; ++rt) {
-    const int live = rows - tile.row0 - rt * 16 < 16 ? rows - tile.row0 - rt * 16 : 16;  // rows that exist
-#pragma unroll 1
-    for (int i0 = 0; i0 < live; i0 += 2 * RI) {
-      float2 ml[2];
-      f32x4 acc[2];
-      int row[2];
+
+  // In a tile's last block, join the parts: a wave takes sets of RI rows, four values a lane, and all
+  // parts of a set if there are sets for every wave, else every `share`-th of them.
+  constexpr int RI = 256 / D, LR = 64 / RI, BATCH = 8;  // rows of a set, lanes a row, parts read at once
+  const int sets = (live + RI - 1) / RI, share = sets >= NW ? 1 : NW / sets, sub = wave % share;
+  f32x4* joined = reinterpret_cast<f32x4*>(&s_o[0][0][0]);  // [share][sets][64]
+  float2* joined_ml = reinterpret_cast<float2*>(joined + NW * 64);
+  const int dl = (lane % LR) * 4;
+  auto give = [&](int r, f32x4 v, float all) {
+    if (r >= live) return;
+    const float inv = all == 0.f ? 0.f : 1.f / all;
+    const float w[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+    store_values<T, 4>(out_at(r) + dl, w);
+  };
+  for (int set = wave / share; set < sets; set += NW / share) {
+    const int r = set * RI + lane / LR;
+    float2 ml = {-__builtin_inff(), 0.f};
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int c0 = sub; c0 < tile.parts; c0 += BATCH * share) {
+      float2 pm[BATCH];
+      f32x4 po[BATCH];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        ml[i] = {-__builtin_inff(), 0.f};
-        acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        row[i] = i0 + i * RI + lane / LR;
+      for (int c = 0; c < BATCH; ++c) {
+        const int part = c0 + c * share;
+        const bool in = part < tile.parts;  // no bytes otherwise
+        const int64_t at = part_row(in ? part : 0);
+        pm[c] = get2(shared_at(a.part_ml + at, in ? 8 * live : 0), r * 8);
+        po[c] = get4(shared_at(a.part_o + at * D, in ? 4 * D * live : 0), (r * D + dl) * 4);
       }
-      for (int c0 = wave; c0 < tile.parts; c0 += 4 * NW) {
-        float2 pm[4][2];
-        f32x4 po[4][2];
+      float to = ml.x;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const bool in = c0 + c * NW < tile.parts;
-          const int64_t at = part_rows(in ? c0 + c * NW : c0) + rt * 16;
-          const auto ro = shared_at(a.part_o + at * D, in ? 4 * D * live : 0);
-          const auto rm = shared_at(a.part_ml + at, in ? 8 * live : 0);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            pm[c][i] = get2(rm, row[i] * 8);
-            po[c][i] = get4(ro, (row[i] * D + (lane % LR) * 4) * 4);
-          }
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (c0 + c * NW >= tile.parts) continue;
-            const float to = max_of(ml[i].x, pm[c][i].x), base = to == -__builtin_inff() ? 0.f : to;
-            const float f0 = __builtin_amdgcn_exp2f(ml[i].x - base), f1 = __builtin_amdgcn_exp2f(pm[c][i].x - base);
-            ml[i] = {to, ml[i].y * f0 + pm[c][i].y * f1};
-            acc[i] = acc[i] * f0 + po[c][i] * f1;
-          }
+      for (int c = 0; c < BATCH; ++c) {
+        if (c0 + c * share >= tile.parts) pm[c].x = -__builtin_inff();
+        to = max_of(to, pm[c].x);
       }
+      const float base = to == -__builtin_inff() ? 0.f : to, f = __builtin_amdgcn_exp2f(ml.x - base);
+      ml = {to, ml.y * f};
+      acc *= f;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if (row[i] >= 16) continue;
-        if (lane % LR == 0) s_ml[wave][row[i]] = ml[i];
-        *reinterpret_cast<f32x4*>(&s_o[wave][row[i]][(lane % LR) * 4]) = acc[i];
+      for (int c = 0; c < BATCH; ++c) {
+        const float g = __builtin_amdgcn_exp2f(pm[c].x - base);
+        ml.y = __builtin_fmaf(pm[c].y, g, ml.y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(po[c][e], g, acc[e]);
       }
     }
-    float v[C], top, all;
-    join(rt, v, top, all);
-    finish(rt, v, all);
+    if (share == 1) {
+      give(r, acc, ml.y);
+    } else {
+      joined[(sub * sets + set) * 64 + lane] = acc;
+      joined_ml[(sub * sets + set) * 64 + lane] = ml;
+    }
+  }
+  if (share == 1) return;
+  __syncthreads();
+  if (wave < sets) {  // fewer than the waves
+    float2 ml = {-__builtin_inff(), 0.f};
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < share; ++u) ml.x = max_of(ml.x, joined_ml[(u * sets + wave) * 64 + lane].x);
+    const float base = ml.x == -__builtin_inff() ? 0.f : ml.x;
+    for (int u = 0; u < share; ++u) {
+      const float2 pm = joined_ml[(u * sets + wave) * 64 + lane];
+      const float g = __builtin_amdgcn_exp2f(pm.x - base);
+      ml.y = __builtin_fmaf(pm.y, g, ml.y);
+      acc += joined[(u * sets + wave) * 64 + lane] * g;
+    }
+    give(wave * RI + lane / LR, acc, ml.y);
   }
 }
 
@@ -1255,6 +1281,7 @@ constexpr int kFewRows = 32;
 struct Plan {
   int rt;           // 16-row tiles of k_attend_few, 0: not used
   bool rows;        // k_attend_rows runs
+  bool ahead;       // k_attend_few: few steps in all
   int64_t grid_few, grid_rows;
   int fill_few, fill_rows;  // blocks that parts fill, 0: no parts
 };
@@ -1271,12 +1298,14 @@ void plan_grid(int64_t T, int64_t B, int Hkv, int grp, int R, int want, int64_t&
   grid = tiles + (fill ? fill + Hkv : 0);
 }
 
-Plan plan_of(bool wide, int64_t T, int64_t B, int Hkv, int grp, int64_t max_query) {
+Plan plan_of(bool wide, int64_t T, int64_t B, int Hkv, int grp, int64_t max_query, int64_t max_context) {
   Plan p{};
   const int64_t rows = (max_query < T ? max_query : T) * grp;  // of a request
   // wide: fp32 heads of 256, of which three parts of 32 queries pass the registers
   p.rt = rows > 16 && !wide ? 2 : 1;
   p.rows = rows > kFewRows && !wide;
+  // 256 blocks of 8 waves, four steps each
+  p.ahead = B * Hkv * cdiv(max_context, 32) <= 8192;
   if (p.rows && B <= 1) p.rt = 0;
   if (p.rt) plan_grid(T, B, Hkv, grp, 16 * p.rt, kFill, p.grid_few, p.fill_few);
   if (p.rows) plan_grid(T, B, Hkv, grp, 128, kFill, p.grid_rows, p.fill_rows);
@@ -1312,19 +1341,30 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
     a.part_ml = reinterpret_cast<float2*>(a.part_o + p.grid_few * 16 * p.rt * D);
     a.rows_from = 0;
     a.rows_upto = p.rows ? kFewRows : 0x7fffffff;
-    a.least = 32;
-    a.whole = 64;
-    auto go = [&](auto rt) {
+    auto go = [&](auto rt, auto ahead) {
       constexpr int RT = decltype(rt)::value;
-      static_assert(kFewFill<T, D, RT> <= kFill);
-      a.blocks = p.fill_few ? kFewFill<T, D, RT> : 0;
-      hipLaunchKernelGGL((k_attend_few<T, D, RT>), dim3((unsigned)p.grid_few), dim3(64 * kFewBlock<T, D, RT>), 0, s,
+      constexpr bool AHEAD = decltype(ahead)::value;
+      static_assert(kFewFill<T, D, RT, AHEAD> <= kFill);
+      a.blocks = p.fill_few ? kFewFill<T, D, RT, AHEAD> : 0;
+      a.least = 16;
+      a.whole = 32;
+      hipLaunchKernelGGL((k_attend_few<T, D, RT, AHEAD>), dim3((unsigned)p.grid_few), dim3(64 * kFewBlock<T, D, RT>), 0, s,
                          a.starts, a.context, a.T, a.B, a.Hkv, a.grp, a.reach, a.window, a.blocks, a);
     };
-    if (p.rt == 1)
-      go(std::integral_constant<int, 1>{});
-    else if constexpr (!wide)
-      go(std::integral_constant<int, 2>{});
+    std::integral_constant<int, 1> one;
+    std::integral_constant<int, 2> two;
+    if (p.rt == 1 || wide) {
+      if constexpr (kFewWaves<T, D, 1, false> > kFewWaves<T, D, 1, true>) {
+        if (p.ahead)
+          go(one, std::true_type{});
+        else
+          go(one, std::false_type{});
+      } else {
+        go(one, std::bool_constant<!kFewWide<T, D, 1> && !(D == 256)>{});
+      }
+    } else if constexpr (!wide) {
+      go(two, std::bool_constant<!kFewWide<T, D, 2>>{});
+    }
   }
   return hip_check(hipGetLastError(), "k_attend launch");
 }
@@ -1352,10 +1392,10 @@ using namespace qs;
 
 extern "C" size_t qs_kv4_attend_workspace_bytes(int64_t T, int64_t B, int Hkv, int Hq, int D, int64_t page_size,
                                                 int64_t max_query, int64_t max_context, int64_t window) {
-  (void)max_context, (void)window;
+  (void)window;
   if (check_sizes(T, B, Hkv, Hq, D, page_size) != QS_OK) return 0;
-  const size_t narrow = space_of(plan_of(false, T, B, Hkv, Hq / Hkv, max_query), D);
-  const size_t wide = D == 256 ? space_of(plan_of(true, T, B, Hkv, Hq / Hkv, max_query), D) : 0;
+  const size_t narrow = space_of(plan_of(false, T, B, Hkv, Hq / Hkv, max_query, max_context), D);
+  const size_t wide = D == 256 ? space_of(plan_of(true, T, B, Hkv, Hq / Hkv, max_query, max_context), D) : 0;
   return narrow > wide ? narrow : wide;
 }
 
@@ -1377,7 +1417,7 @@ extern "C" int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ld
   if (ldq_t % per16 || ldq_h % per16 || !aligned(q, 16) || !aligned(out, 16) || !aligned(cache, 16))
     return fail(QS_ERR_INVALID, "kv4_attend: 16-byte alignment");
   const int grp = Hq / Hkv;
-  const Plan p = plan_of(dtype == QS_F32 && D == 256, T, B, Hkv, grp, max_query);
+  const Plan p = plan_of(dtype == QS_F32 && D == 256, T, B, Hkv, grp, max_query, max_context);
   const size_t need = space_of(p, D);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QS_ERR_INVALID, "kv4_attend: workspace of qs_kv4_attend_workspace_bytes() bytes, 16-byte aligned");
