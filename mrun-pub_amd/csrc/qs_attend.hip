@@ -177,7 +177,7 @@ constexpr float kSlack = 8.f;
 // ---- which rows and tokens a block has -----------------------------------------------------
 struct Work {
   int64_t q0;         // first token of the request
-  int b, n, row0;     // request, its new tokens, first row of the tile
+  int b, n, ctx, row0;  // request, its new tokens and context, first row of the tile
   int part, parts;    // which part of the tile's tokens, of how many
   int64_t first;      // block of the tile's part 0
   int hk;
@@ -201,21 +201,34 @@ __device__ __forceinline__ bool mine(const AttendArgs& a, int rows) { return row
 
 // Without parts: request b's tiles of R rows start at floor(starts[b] grp / R) + b, which leaves each
 // request room for its last, partial one and can be searched without sums over requests.
-__device__ __forceinline__ Work pick_tile(const AttendArgs& a, int64_t y, int R) {
+template <int R>
+__device__ __forceinline__ Work pick_tile(const AttendArgs& a, int64_t y) {
   const int lane = threadIdx.x & 63;
-  int at = -1;
-  for (int b0 = 0; b0 <= a.B; b0 += 64) {
-    const int b = b0 + lane;
-    const bool before = b <= a.B && (int64_t)((uint64_t)(start_of(a, b) * a.grp) / (unsigned)R) + b <= y;
-    const int n = __popcll(__ballot(before));
-    at += n;
-    if (n < 64) break;
-  }
   Work t;
-  t.b = at;
-  t.q0 = start_of(a, at);
-  t.n = new_of(a, at, t.q0);
-  int64_t tile = y - ((int64_t)((uint64_t)(t.q0 * a.grp) / (unsigned)R) + at);
+  int64_t tile;
+  if (a.B < 64) {  // a lane a request (and one for the tokens after them): one round trip
+    const int start = lane <= a.B ? (int)start_of(a, lane) : 0, ctx = lane <= a.B ? context_of(a, lane) : 0;
+    const bool before = lane <= a.B && (int64_t)((uint64_t)((int64_t)start * a.grp) / R) + lane <= y;
+    t.b = __popcll(__ballot(before)) - 1;
+    t.q0 = __builtin_amdgcn_readlane(start, t.b);
+    const int q1 = t.b < a.B ? __builtin_amdgcn_readlane(start, t.b + 1) : a.T;
+    t.n = q1 > t.q0 ? q1 - (int)t.q0 : 0;
+    t.ctx = __builtin_amdgcn_readlane(ctx, t.b);
+  } else {
+    int at = -1;
+    for (int b0 = 0; b0 <= a.B; b0 += 64) {
+      const int b = b0 + lane;
+      const bool before = b <= a.B && (int64_t)((uint64_t)(start_of(a, b) * a.grp) / R) + b <= y;
+      const int n = __popcll(__ballot(before));
+      at += n;
+      if (n < 64) break;
+    }
+    t.b = at;
+    t.q0 = start_of(a, at);
+    t.n = new_of(a, at, t.q0);
+    t.ctx = context_of(a, at);
+  }
+  tile = y - ((int64_t)((uint64_t)(t.q0 * a.grp) / R) + t.b);
   const int64_t tiles = ((int64_t)t.n * a.grp + R - 1) / R;
   t.any = tile >= 0 && tile < tiles && mine(a, t.n * a.grp);
   t.row0 = (int)((tiles - 1 - tile) * R);  // the last rows see most: they start first
@@ -252,13 +265,13 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
   const int me = alone ? lane : threadIdx.x, each = alone ? 1 : a.B / THREADS + 1;  // of B + 1 requests
   const int b0 = me * each < a.B + 1 ? me * each : a.B + 1, b1 = b0 + each < a.B + 1 ? b0 + each : a.B + 1;
   int64_t q0 = 0;
-  int n = 0, tiles = 0, steps = 0;
+  int n = 0, ctx = 0, tiles = 0, steps = 0;
   auto look = [&](int b) {
     q0 = start_of(a, b);
     n = new_of(a, b, q0);
     const int rows = n * a.grp;
     tiles = mine(a, rows) ? (rows + R - 1) / R : 0;
-    const int ctx = context_of(a, b);
+    ctx = context_of(a, b);
     int span = ctx < a.reach ? ctx : a.reach;
     if (a.window > 0 && span > a.window + R) span = a.window + R;  // of one tile
     steps = (span + STEP - 1) / STEP;
@@ -323,6 +336,7 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
     t.b = from;
     t.q0 = (int64_t)__builtin_amdgcn_readlane((int)q0, from);  // below 2^31
     t.n = __builtin_amdgcn_readlane(n, from);
+    t.ctx = __builtin_amdgcn_readlane(ctx, from);
     before = __builtin_amdgcn_readlane(before, from);
     tiles = __builtin_amdgcn_readlane(tiles, from);
     t.parts = __builtin_amdgcn_readlane(parts_for(per_step), from);
@@ -340,6 +354,7 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
           t.q0 = q0;
           t.b = b;
           t.n = n;
+          t.ctx = ctx;
           t.row0 = (tiles - 1 - tile) * R;
           t.part = y - before - tile * parts;
           t.parts = parts;
@@ -360,10 +375,11 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
 template <int R, int STEP, int THREADS>
 __device__ __forceinline__ Work pick_work(const AttendArgs& a, float* s_sum, Work* s_work) {
   const unsigned x = blockIdx.x, y = x / (unsigned)a.Hkv;  // heads side by side: each to its own XCD's cache
-  Work t = a.blocks > 0 ? pick_part<R, STEP, THREADS>(a, (int)y, s_sum, s_work) : pick_tile(a, y, R);
+  Work t = a.blocks > 0 ? pick_part<R, STEP, THREADS>(a, (int)y, s_sum, s_work) : pick_tile<R>(a, y);
   t.hk = (int)(x - y * (unsigned)a.Hkv);
   t.b = __builtin_amdgcn_readfirstlane(t.b);
   t.n = __builtin_amdgcn_readfirstlane(t.n);
+  t.ctx = __builtin_amdgcn_readfirstlane(t.ctx);
   t.row0 = __builtin_amdgcn_readfirstlane(t.row0);
   t.part = __builtin_amdgcn_readfirstlane(t.part);
   t.parts = __builtin_amdgcn_readfirstlane(t.parts);
@@ -473,23 +489,33 @@ __device__ __forceinline__ bool last_part(const AttendArgs& a, const Work& w, in
 }
 
 // ---- few rows --------------------------------------------------------------------------------
-// AHEAD: registers hold the next step's codes too, which hides a load's time where few waves run;
-// the other form leaves room for twice the waves where their number does that.
-template <class T, int D, int RT>
-constexpr bool kFewWide = kCodes<T> ? D * RT >= 256 : D * RT >= 512;
-template <class T, int D, int RT, bool AHEAD>
-constexpr int kFewWaves = kFewWide<T, D, RT> ? 1 : !AHEAD && D * RT * kParts<T> <= 192 ? 4 : 2;  // a SIMD
-template <class T, int D, int RT>
-constexpr int kFewBlock = kFewWide<T, D, RT> ? 4 : 8;  // waves of a block
-template <class T, int D, int RT, bool AHEAD>
-constexpr int kFewFill = 1024 * kFewWaves<T, D, RT, AHEAD> / kFewBlock<T, D, RT>;  // blocks that run at once
+// ahead: registers hold the next step's codes too, which hides a load's time where few waves run; the
+// other form leaves room for twice the waves where their number does that, in blocks of half the
+// size, which share out ragged requests more evenly.
+constexpr bool few_wide(bool codes, int D, int rt) { return D * rt >= (codes ? 256 : 512); }
+constexpr int few_waves(bool codes, int D, int rt, bool ahead) {  // a SIMD, as the registers allow
+  return few_wide(codes, D, rt) ? 1 : !ahead && D * rt * (codes ? 3 : 1) <= 192 ? 4 : 2;
+}
+constexpr int few_block(bool codes, int D, int rt, bool ahead) {  // waves of a block
+  return few_wide(codes, D, rt) || !ahead ? 4 : 8;
+}
+constexpr int few_fill(bool codes, int D, int rt, bool ahead) {  // blocks that run at once
+  return 1024 * few_waves(codes, D, rt, ahead) / few_block(codes, D, rt, ahead);
+}
+// Where both forms exist, `few steps` takes the first.
+constexpr bool few_ahead(bool codes, int D, int rt, bool few_steps) {
+  if (few_wide(codes, D, rt) || D == 256) return false;
+  return few_steps || few_waves(codes, D, rt, false) == few_waves(codes, D, rt, true);
+}
+constexpr int kFewLeast = 16, kFewWhole = 32;    // steps of a part at least, steps that stay whole
+constexpr int kRowsLeast = 4, kRowsWhole = 8, kRowsFill = 512;
 
 template <class T, int D, int RT, bool AHEAD>
-__global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT, AHEAD>)) void k_attend_few(
+__global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_waves(kCodes<T>, D, RT, AHEAD))) void k_attend_few(
     const int* starts, const int* context, int tokens, int requests, int Hkv, int grp, int reach, int window, int blocks, AttendArgs a) {
   a.starts = starts, a.context = context, a.T = tokens, a.B = requests, a.Hkv = Hkv, a.grp = grp, a.reach = reach;
   a.window = window, a.blocks = blocks;
-  constexpr int NW = kFewBlock<T, D, RT>;
+  constexpr int NW = few_block(kCodes<T>, D, RT, AHEAD);
   using O = Ops<T>;
   typedef typename O::Frag Frag;
   constexpr int G = D / kKv4Group, KS = D / 32, R = 16 * RT, W = 2 * G, NP = kParts<T>;
@@ -504,7 +530,7 @@ __global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT, AH
   const Work tile = pick_work<R, 32, 64 * NW>(a, s_sum, &s_work);
   if (!tile.any) return;
   const int hk = tile.hk, rows = tile.n * a.grp;
-  const int past = context_of(a, tile.b) - tile.n;  // position of the first new token
+  const int past = tile.ctx - tile.n;  // position of the first new token
   const int r_last = tile.row0 + R - 1 < rows ? tile.row0 + R - 1 : rows - 1;
   const int pos_min = past + tile.row0 / a.grp, pos_max = past + r_last / a.grp;
   const Span span = span_of(a, tile.b, pos_min, pos_max);
@@ -835,7 +861,7 @@ __global__ __launch_bounds__((64 * kFewBlock<T, D, RT>), (kFewWaves<T, D, RT, AH
 
   // In a tile's last block, join the parts: a wave takes sets of RI rows, four values a lane, and all
   // parts of a set if there are sets for every wave, else every `share`-th of them.
-  constexpr int RI = 256 / D, LR = 64 / RI, BATCH = 8;  // rows of a set, lanes a row, parts read at once
+  constexpr int RI = 256 / D, LR = 64 / RI, BATCH = 64 / NW;  // rows of a set, lanes a row, parts read at once
   const int sets = (live + RI - 1) / RI, share = sets >= NW ? 1 : NW / sets, sub = wave % share;
   f32x4* joined = reinterpret_cast<f32x4*>(&s_o[0][0][0]);  // [share][sets][64]
   float2* joined_ml = reinterpret_cast<float2*>(joined + NW * 64);
@@ -941,7 +967,7 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
   const Work tile = pick_work<R, TT, 256>(a, s_sum, &s_work);
   if (!tile.any) return;
   const int hk = tile.hk, rows = tile.n * a.grp;
-  const int past = context_of(a, tile.b) - tile.n;
+  const int past = tile.ctx - tile.n;
   const int r_last = tile.row0 + R - 1 < rows ? tile.row0 + R - 1 : rows - 1;
   const Span span = span_of(a, tile.b, past + tile.row0 / a.grp, past + r_last / a.grp);
   const int lo = span.lo, hi = span.hi;
@@ -1277,38 +1303,45 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
 
 // ---- launch -------------------------------------------------------------------------------
 constexpr int kFewRows = 32;
+constexpr int kSyncWords = 8192;  // of the workspace's start, one a block
 
 struct Plan {
   int rt;           // 16-row tiles of k_attend_few, 0: not used
   bool rows;        // k_attend_rows runs
-  bool ahead;       // k_attend_few: few steps in all
+  bool ahead;       // which form of k_attend_few
   int64_t grid_few, grid_rows;
   int fill_few, fill_rows;  // blocks that parts fill, 0: no parts
 };
 
-// Blocks of one kernel, R rows a tile: a block a tile and head, and with parts `want` more.  Tiles in
-// thousands fill the chip without parts, and the sums over many requests would cost every block more.
-constexpr int kSyncWords = 8192;  // of the workspace's start, one a block
-constexpr int kFill = 512;        // blocks that parts fill, at most
-
-void plan_grid(int64_t T, int64_t B, int Hkv, int grp, int R, int want, int64_t& grid, int& fill) {
+// Blocks of one kernel, R rows a tile: a block a tile and head, and with parts `fill` more, if by the
+// caller's bounds some tile has more steps than stay whole.  Tiles in thousands fill the chip without
+// parts, and the sums over many requests would cost every block more.
+void plan_grid(int64_t T, int64_t B, int Hkv, int grp, int R, int64_t rows, int64_t steps, int whole, int least, int most,
+               int64_t& grid, int& fill) {
   const int64_t tiles = (T * grp / R + B + 1) * Hkv;
-  fill = tiles <= 4 * want && B < 1024 ? want : 0;
-  if (fill && tiles + fill + Hkv > kSyncWords) fill = 0;
+  const int64_t likely = cdiv(rows, R) * B * Hkv * cdiv(steps, least);
+  fill = steps > whole && tiles <= 4 * most && B < 1024 ? (int)(likely < most ? likely : most) : 0;
+  if (tiles + fill + Hkv > kSyncWords) fill = 0;
   grid = tiles + (fill ? fill + Hkv : 0);
 }
 
-Plan plan_of(bool wide, int64_t T, int64_t B, int Hkv, int grp, int64_t max_query, int64_t max_context) {
+Plan plan_of(bool codes, int D, int64_t T, int64_t B, int Hkv, int grp, int64_t max_query, int64_t max_context, int64_t window) {
   Plan p{};
   const int64_t rows = (max_query < T ? max_query : T) * grp;  // of a request
-  // wide: fp32 heads of 256, of which three parts of 32 queries pass the registers
+  int64_t span = max_context;
+  if (window > 0 && span > window + 128) span = window + 128;
+  const bool wide = codes && D == 256;  // three parts of 32 such queries pass the registers
   p.rt = rows > 16 && !wide ? 2 : 1;
   p.rows = rows > kFewRows && !wide;
-  // 256 blocks of 8 waves, four steps each
-  p.ahead = B * Hkv * cdiv(max_context, 32) <= 8192;
+  p.ahead = few_ahead(codes, D, p.rt, B * Hkv * cdiv(span, 32) <= 8192);  // 256 blocks of 8 waves, four steps each
+  const int most = few_fill(codes, D, p.rt, p.ahead);
   if (p.rows && B <= 1) p.rt = 0;
-  if (p.rt) plan_grid(T, B, Hkv, grp, 16 * p.rt, kFill, p.grid_few, p.fill_few);
-  if (p.rows) plan_grid(T, B, Hkv, grp, 128, kFill, p.grid_rows, p.fill_rows);
+  if (p.rt)
+    plan_grid(T, B, Hkv, grp, 16 * p.rt, rows < kFewRows ? rows : kFewRows, cdiv(span, 32) + 1, kFewWhole, kFewLeast, most,
+              p.grid_few, p.fill_few);
+  if (p.rows)
+    plan_grid(T, B, Hkv, grp, 128, rows, cdiv(span, D == 256 ? 32 : 64) + 1, kRowsWhole, kRowsLeast, kRowsFill, p.grid_rows,
+              p.fill_rows);
   return p;
 }
 
@@ -1328,8 +1361,8 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
       a.rows_from = p.rt ? kFewRows + 1 : 0;
       a.rows_upto = 0x7fffffff;
       a.blocks = p.fill_rows;
-      a.least = 4;
-      a.whole = 8;
+      a.least = kRowsLeast;
+      a.whole = kRowsWhole;
       const size_t lds = 2 * sizeof(RowsTile<T, D>);
       static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attend_rows<T, D>),
                                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -1341,29 +1374,30 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
     a.part_ml = reinterpret_cast<float2*>(a.part_o + p.grid_few * 16 * p.rt * D);
     a.rows_from = 0;
     a.rows_upto = p.rows ? kFewRows : 0x7fffffff;
+    a.blocks = p.fill_few;
+    a.least = kFewLeast;
+    a.whole = kFewWhole;
     auto go = [&](auto rt, auto ahead) {
       constexpr int RT = decltype(rt)::value;
       constexpr bool AHEAD = decltype(ahead)::value;
-      static_assert(kFewFill<T, D, RT, AHEAD> <= kFill);
-      a.blocks = p.fill_few ? kFewFill<T, D, RT, AHEAD> : 0;
-      a.least = 16;
-      a.whole = 32;
-      hipLaunchKernelGGL((k_attend_few<T, D, RT, AHEAD>), dim3((unsigned)p.grid_few), dim3(64 * kFewBlock<T, D, RT>), 0, s,
-                         a.starts, a.context, a.T, a.B, a.Hkv, a.grp, a.reach, a.window, a.blocks, a);
+      if constexpr (few_ahead(kCodes<T>, D, RT, AHEAD) == AHEAD)  // the forms that a plan takes
+        hipLaunchKernelGGL((k_attend_few<T, D, RT, AHEAD>), dim3((unsigned)p.grid_few),
+                           dim3(64 * few_block(kCodes<T>, D, RT, AHEAD)), 0, s, a.starts, a.context, a.T, a.B, a.Hkv, a.grp,
+                           a.reach, a.window, a.blocks, a);
     };
-    std::integral_constant<int, 1> one;
-    std::integral_constant<int, 2> two;
-    if (p.rt == 1 || wide) {
-      if constexpr (kFewWaves<T, D, 1, false> > kFewWaves<T, D, 1, true>) {
-        if (p.ahead)
-          go(one, std::true_type{});
-        else
-          go(one, std::false_type{});
-      } else {
-        go(one, std::bool_constant<!kFewWide<T, D, 1> && !(D == 256)>{});
-      }
-    } else if constexpr (!wide) {
-      go(two, std::bool_constant<!kFewWide<T, D, 2>>{});
+    auto go_rows = [&](auto rt) {
+      if (p.ahead)
+        go(rt, std::true_type{});
+      else
+        go(rt, std::false_type{});
+    };
+    if constexpr (wide) {
+      go_rows(std::integral_constant<int, 1>{});
+    } else {
+      if (p.rt == 1)
+        go_rows(std::integral_constant<int, 1>{});
+      else
+        go_rows(std::integral_constant<int, 2>{});
     }
   }
   return hip_check(hipGetLastError(), "k_attend launch");
@@ -1392,11 +1426,10 @@ using namespace qs;
 
 extern "C" size_t qs_kv4_attend_workspace_bytes(int64_t T, int64_t B, int Hkv, int Hq, int D, int64_t page_size,
                                                 int64_t max_query, int64_t max_context, int64_t window) {
-  (void)window;
   if (check_sizes(T, B, Hkv, Hq, D, page_size) != QS_OK) return 0;
-  const size_t narrow = space_of(plan_of(false, T, B, Hkv, Hq / Hkv, max_query, max_context), D);
-  const size_t wide = D == 256 ? space_of(plan_of(true, T, B, Hkv, Hq / Hkv, max_query, max_context), D) : 0;
-  return narrow > wide ? narrow : wide;
+  const size_t f16 = space_of(plan_of(false, D, T, B, Hkv, Hq / Hkv, max_query, max_context, window), D);
+  const size_t f32 = space_of(plan_of(true, D, T, B, Hkv, Hq / Hkv, max_query, max_context, window), D);
+  return f16 > f32 ? f16 : f32;
 }
 
 extern "C" int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ldq_h, const uint8_t* cache,
@@ -1417,7 +1450,7 @@ extern "C" int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ld
   if (ldq_t % per16 || ldq_h % per16 || !aligned(q, 16) || !aligned(out, 16) || !aligned(cache, 16))
     return fail(QS_ERR_INVALID, "kv4_attend: 16-byte alignment");
   const int grp = Hq / Hkv;
-  const Plan p = plan_of(dtype == QS_F32 && D == 256, T, B, Hkv, grp, max_query, max_context);
+  const Plan p = plan_of(dtype == QS_F32, D, T, B, Hkv, grp, max_query, max_context, window);
   const size_t need = space_of(p, D);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QS_ERR_INVALID, "kv4_attend: workspace of qs_kv4_attend_workspace_bytes() bytes, 16-byte aligned");

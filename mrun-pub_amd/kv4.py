@@ -142,7 +142,7 @@ def read(cache: KV4Cache, layer: int, slots: torch.Tensor, *,
 
 @functools.lru_cache(maxsize=512)
 def _attend_space(*sizes: int) -> int:
-    return int(nat.load().qs_kv4_attend_workspace_bytes(*sizes, 0, 0))
+    return int(nat.load().qs_kv4_attend_workspace_bytes(*sizes))
 
 
 @nat.inference
@@ -184,6 +184,8 @@ def attend(
     most = width * cache.page_size
     mq = T if max_query is None else int(max_query)
     mc = most if max_context is None else min(int(max_context), most)
+    mc = -(-mc // 512) * 512  # so that a step's plan serves the next steps
+    win = int(window or 0)
     if mq < 0 or mc < 0 or (window is not None and window < 1):
         raise ValueError("bounds must not be negative and a window holds at least one token")
     s = 1.0 / math.sqrt(D) if scale is None else float(scale)
@@ -196,11 +198,11 @@ def attend(
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous() or out.data_ptr() % 16:
         raise ValueError("attention output must be contiguous, 16-byte aligned, of the queries' shape and type")
     stream = nat.stream_of(device)
-    need = _attend_space(T, B, cache.kv_heads, Hq, D, cache.page_size, mq)
+    need = _attend_space(T, B, cache.kv_heads, Hq, D, cache.page_size, mq, mc, win)
     workspace = nat.kept_workspace(device, stream, need) if need else None
     nat.call(
         "qs_kv4_attend", nat.ptr(q), nat.dtype_code(q.dtype), q.stride(0), q.stride(1), base, cache.pages,
         cache.page_size, cache.kv_heads, Hq, D, nat.ptr(block_tables), block_tables.stride(0), width, nat.ptr(starts),
-        nat.ptr(ctx), B, T, mq, mc, s, int(window or 0), nat.ptr(out), nat.ptr(workspace), need, stream,
+        nat.ptr(ctx), B, T, mq, mc, s, win, nat.ptr(out), nat.ptr(workspace), need, stream,
     )
     return out
