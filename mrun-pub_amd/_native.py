@@ -185,24 +185,25 @@ def inference(fn):
     return run
 
 
-_kept: dict[tuple[int, int], torch.Tensor] = {}
-SYNC_BYTES = 32768  # of a workspace's start, in which kernels count their blocks
+_fast = None
+# the C entry points that the binding module calls, in its order
+_FAST = ("qs_plan_step", "qs_rotary", "qs_kv4_append", "qs_kv4_read", "qs_kv4_attend", "qs_kv4_attend_workspace_bytes",
+         "qs_last_error")
 
 
-def kept_workspace(device: torch.device, stream: int, need: int) -> torch.Tensor:
-    """A workspace whose first ``SYNC_BYTES`` are zero, for kernels that leave them zero: one a
-    stream, whose calls follow one another.  A call that is captured into a graph, which may run
-    beside them, gets one of its own, cleared in the graph."""
-    if torch.cuda.is_current_stream_capturing():
-        fresh = torch.empty(need, dtype=torch.uint8, device=device)
-        fresh[:SYNC_BYTES].zero_()
-        return fresh
-    have = _kept.get((device.index, stream))
-    if have is None or have.numel() < need:
-        have = torch.empty(need, dtype=torch.uint8, device=device)
-        have[:SYNC_BYTES].zero_()
-        _kept[device.index, stream] = have
-    return have
+def fast():
+    """The binding module of the operators whose calls have to be short (checks, allocations and the
+    launch in one native call).  Raises RuntimeError if it is not built."""
+    global _fast
+    if _fast is None:
+        lib = load()
+        try:
+            from . import _qs_torch as module
+        except ImportError as exc:
+            raise RuntimeError("QStore torch binding not built; run __graft_entry__.build()") from exc
+        module.bind(*(ctypes.cast(getattr(lib, name), _P).value for name in _FAST))
+        _fast = module
+    return _fast
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -1,4 +1,5 @@
-"""Build ``libqstore_hip.so`` (the gfx950 kernels + C ABI) in-tree with hipcc.
+"""Build ``libqstore_hip.so`` (the gfx950 kernels + C ABI) in-tree with hipcc, and ``_qs_torch.so``
+(host code: the torch binding of the operators whose calls have to be short) with g++.
 
 Usage: ``python mrun-pub_amd/build.py`` or ``build()`` from Python.  Objects go to
 ``mrun-pub_amd/_build/``; the shared library lands next to this file so it travels
@@ -19,6 +20,7 @@ PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 BUILD_DIR = PKG_DIR / "_build"
 LIB_NAME = "libqstore_hip.so"
+BINDING_NAME = "_qs_torch.so"
 LIB_PATH = PKG_DIR / LIB_NAME
 ARCH = "gfx950"
 
@@ -82,14 +84,38 @@ def _compile(src: Path) -> Path:
     return obj
 
 
+def _build_binding() -> Path:
+    """Compile the torch binding, a plain CPython module against torch's headers and libraries."""
+    import sysconfig
+
+    import torch
+
+    home, out = Path(torch.__file__).resolve().parent, PKG_DIR / BINDING_NAME
+    tmp = out.with_suffix(".so.tmp")
+    cmd = [
+        os.environ.get("CXX", "g++"), "-O2", "-fPIC", "-shared", "-std=c++17", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", str(home / "include"), "-isystem",
+        str(home / "include/torch/csrc/api/include"), "-isystem", str(Path(HIPCC).resolve().parent.parent / "include"),
+        "-isystem", sysconfig.get_paths()["include"], str(CSRC / "binding" / "qs_torch.cpp"), "-o", str(tmp),
+        f"-L{home / 'lib'}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python", f"-Wl,-rpath,{home / 'lib'}",
+    ]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"torch binding failed:\n{proc.stderr}")
+    os.replace(tmp, out)
+    return out
+
+
 def build(verbose: bool = False) -> Path:
-    """Compile every HIP/C++ source and link the shared library; returns its path."""
+    """Compile every HIP/C++ source and link the libraries; returns the kernels' path."""
     if not Path(HIPCC).exists() and shutil.which("hipcc") is None:
         raise RuntimeError("hipcc not found: the QStore HIP library cannot be built")
     BUILD_DIR.mkdir(exist_ok=True)
     sources = _sources()
-    with ThreadPoolExecutor(max_workers=min(8, len(sources))) as pool:
+    with ThreadPoolExecutor(max_workers=min(8, len(sources) + 1)) as pool:
+        binding = pool.submit(_build_binding)
         objs = list(pool.map(_compile, sources))
+        binding.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     proc = subprocess.run(cmd, capture_output=True, text=True)

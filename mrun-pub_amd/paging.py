@@ -10,7 +10,7 @@ graph, and nothing waits for the GPU.
 
 from __future__ import annotations
 
-from dataclasses import dataclass
+from typing import NamedTuple
 
 import torch
 
@@ -25,8 +25,7 @@ def free_pages(pages: int, device, *, first: int = 0) -> tuple[torch.Tensor, tor
     return ring, torch.tensor([0, pages - first, 0], dtype=torch.int64, device=device)
 
 
-@dataclass(frozen=True)
-class StepPlan:
+class StepPlan(NamedTuple):
     """One step's metadata; every tensor is on the device.
 
     ``slots [tokens] int64`` (page * page_size + offset; -1 for a row of padding or one whose page
@@ -62,7 +61,6 @@ def _lengths(name: str, lens: torch.Tensor, requests: int) -> torch.Tensor:
     return lens.to(torch.int32).contiguous()
 
 
-@nat.inference
 def plan_step(
     ring: torch.Tensor, free_state: torch.Tensor, block_tables: torch.Tensor, past_lens: torch.Tensor,
     new_lens: torch.Tensor, *, page_size: int, tokens: int,
@@ -76,24 +74,9 @@ def plan_step(
     the new tokens are left out, their pages and context too.  Columns past the table's width take
     no pages.
     """
-    _pool(ring, free_state)
-    B, T = int(past_lens.numel()), int(tokens)
-    past, new = _lengths("past_lens", past_lens, B), _lengths("new_lens", new_lens, B)
-    _tables(block_tables, B)
-    if T < 0:
-        raise ValueError("tokens must not be negative")
-    device = nat.require_device(ring, free_state, block_tables, past, new)
-    slots = torch.empty(T, dtype=torch.int64, device=device)
-    words = torch.empty(2 * T + 2 * B + 1, dtype=torch.int32, device=device)
-    positions, requests, starts, context = words.split([T, T, B + 1, B])
-    state = torch.empty(3, dtype=torch.int64, device=device)
-    nat.call(
-        "qs_plan_step", nat.ptr(ring), int(ring.numel()), nat.ptr(free_state), nat.ptr(state), nat.ptr(block_tables),
-        block_tables.stride(0), int(block_tables.shape[1]), nat.ptr(past), nat.ptr(new), B, int(page_size), T,
-        nat.ptr(slots), nat.ptr(positions), nat.ptr(requests), nat.ptr(starts), nat.ptr(context),
-        nat.stream_of(device),
+    return StepPlan._make(
+        nat.fast().plan_step(ring, free_state, block_tables, past_lens, new_lens, page_size, tokens)
     )
-    return StepPlan(slots, positions, requests, starts, context, state)
 
 
 @nat.inference

@@ -40,10 +40,12 @@ class RotarySpec:
         if not base > 0 or not math.isfinite(base):
             raise ValueError("the rotary base must be positive and finite")
         self.dim, self.base, self.layout = int(dim), float(base), layout
+        self.interleaved = layout == "interleaved"
         self.scaling = dict(scaling) if scaling else None
         self.magnitude = 1.0
         index = torch.arange(dim // 2, dtype=torch.float64)
         self.frequencies = self._frequencies(index)
+        self.native = (self.dim, self.interleaved, self.magnitude)  # as the binding takes a spec
         self._on: dict[torch.device, torch.Tensor] = {}
 
     def _frequencies(self, index: torch.Tensor) -> torch.Tensor:
@@ -89,16 +91,6 @@ class RotarySpec:
         return f
 
 
-def check_positions(positions: torch.Tensor, tokens: int) -> torch.Tensor:
-    """``positions`` as the contiguous int32 vector that the kernels read."""
-    if positions.ndim != 1 or int(positions.numel()) != tokens:
-        raise ValueError("positions must be one per token")
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError("positions must be int32 or int64")
-    return positions.to(torch.int32).contiguous()
-
-
-@nat.inference
 def apply_rotary(
     x: torch.Tensor, positions: torch.Tensor, spec: RotarySpec, *, inverse: bool = False,
     out: torch.Tensor | None = None,
@@ -110,25 +102,5 @@ def apply_rotary(
     ``inverse=True`` turns back, which is also the gradient: with respect to x, of a loss whose
     gradient with respect to the result is given.  ``out`` may be ``x`` itself.
     """
-    if x.ndim != 3:
-        raise ValueError("rotary input must have shape [tokens, heads, head_dim]")
-    T, H, D = map(int, x.shape)
-    if spec.dim > D:
-        raise ValueError(f"rotary spec turns {spec.dim} values of a head of {D}")
-    code = nat.dtype_code(x.dtype)
-    pos = check_positions(positions, T)
-    device = nat.require_device(x, pos, out)
-    if x.stride(2) != 1:
-        x = x.contiguous()
-    if out is None:
-        out = torch.empty((T, H, D), dtype=x.dtype, device=device)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.stride(2) != 1:
-        raise ValueError("rotary output must have the input's shape and type, with contiguous heads")
-    if T == 0 or H == 0:
-        return out
-    nat.call(
-        "qs_rotary", nat.ptr(x), code, x.stride(0), x.stride(1), nat.ptr(pos), nat.ptr(spec.on(device)), spec.dim,
-        int(spec.layout == "interleaved"), int(bool(inverse)), spec.magnitude, nat.ptr(out), out.stride(0),
-        out.stride(1), T, H, D, nat.stream_of(device),
-    )
-    return out
+    freq = spec.on(x.device) if x.is_cuda else None
+    return nat.fast().rotary(x, positions, freq, spec.dim, spec.interleaved, inverse, spec.magnitude, out)
