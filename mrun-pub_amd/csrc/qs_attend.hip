@@ -149,7 +149,18 @@ __device__ __forceinline__ void parts_of(const float (&v)[8], bf16x8 (&p)[3]) {
   }
 }
 
+// Adds eight weights to l: the rounded ones in pairs where they are fp16, which is what the values are
+// multiplied by.
+__device__ __forceinline__ float add_weights(const float (&)[8], const f16x8 (&p)[1], float l) {
+  const f16x2 one = {(_Float16)1.f, (_Float16)1.f};
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) l = __builtin_amdgcn_fdot2(f16x2{p[0][i], p[0][i + 1]}, one, l, false);
+  return l;
+}
+
 __device__ __forceinline__ float max_of(float a, float b) { return a > b ? a : b; }
+// The larger, NaN if either is: one operation for two more values, and none to quiet its inputs.
+__device__ __forceinline__ float top_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 // Maximum / sum over lanes l and l ^ 32, and over the four of l, l ^ 16, l ^ 32, l ^ 48.
 __device__ __forceinline__ float pair_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -168,6 +179,15 @@ __device__ __forceinline__ float quad_sum(float v) {
   v = pair_sum(v);
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// 2^(score - maximum), the score still to be multiplied by rs.  Codes: multiplied first, so that the score
+// that is the maximum has weight 1 exactly; what code s and lo cancel of each other then loses nothing
+// in a row that sees one token, and in others 2^-24 of the group's range, not of the value.
+template <class T>
+__device__ __forceinline__ float weight_of(float x, float rs, float base) {
+  if constexpr (kCodes<T>) return __builtin_amdgcn_exp2f(x * rs - base);
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(x, rs, -base));
 }
 
 // A maximum is moved only by scores that pass it by 2^8: weights up to 256 lose nothing in fp16 or
@@ -701,27 +721,26 @@ __global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_wav
           for (int r = 0; r < 4; ++r) x[rt][4 * h + r] = sc[rt][r];
       }
     }
-    if constexpr (!AHEAD) {  // the registers of the keys are free: the next step's are under way from here
-      __builtin_amdgcn_sched_barrier(0);
-      load_k(ahead, step + NW, next_k);
-      __builtin_amdgcn_sched_barrier(0);
-    }
     float p[RT][8];
     Frag pf[RT][NP];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (edge) {
+        const int last = pos[rt] < hi - 1 ? pos[rt] : hi - 1, upto = last - t0 - 4 * qq;
+        const int from = a.window > 0 ? pos[rt] - a.window + 1 - t0 - 4 * qq : -(1 << 30);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int t = t0 + 16 * (e >> 2) + 4 * qq + (e & 3);
-          const bool see = t <= pos[rt] && t < hi && (a.window <= 0 || t > pos[rt] - a.window) && !(bad >> (e >> 2) & 1);
-          x[rt][e] = see ? x[rt][e] : -__builtin_inff();
+          const int at = 16 * (e >> 2) + (e & 3);
+          x[rt][e] = (at > upto) | (at < from) ? -__builtin_inff() : x[rt][e];
         }
-      }
-      float top = x[rt][0] *= rs[rt];
+        if (bad)
 #pragma unroll
-      for (int e = 1; e < 8; ++e) top = fmaxf(top, x[rt][e] *= rs[rt]);
-      top = quad_max(top);
+          for (int e = 0; e < 8; ++e) x[rt][e] = bad >> (e >> 2) & 1 ? -__builtin_inff() : x[rt][e];
+      }
+      float top = x[rt][0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) top = top_of(top, x[rt][e]);
+      top = quad_max(top) * rs[rt];
       if (__any(top > m[rt] + kSlack)) {
         const float to = max_of(m[rt], top);
         const float f = to == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m[rt] - to);
@@ -737,10 +756,18 @@ __global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_wav
       const float base = m[rt] == -__builtin_inff() ? 0.f : m[rt];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[rt][e] = __builtin_amdgcn_exp2f(x[rt][e] - base);
-        l[rt] += p[rt][e];
+        p[rt][e] = weight_of<T>(x[rt][e], rs[rt], base);
+        if constexpr (kCodes<T>) l[rt] += p[rt][e];
       }
-      if constexpr (!kCodes<T>) parts_of(p[rt], pf[rt]);
+      if constexpr (!kCodes<T>) {
+        parts_of(p[rt], pf[rt]);
+        l[rt] = add_weights(p[rt], pf[rt], l[rt]);
+      }
+    }
+    if constexpr (!AHEAD) {  // registers of keys and scores are free: the next step's are under way from here
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(ahead, step + NW, next_k);
+      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int g = 0; g < G; ++g) {
@@ -993,16 +1020,17 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
   const int s0 = first + (int)((int64_t)steps * tile.part / tile.parts);
   const int s1 = first + (int)((int64_t)steps * (tile.part + 1) / tile.parts);
   const Kv4Layout L(a.P, D);
-  const int64_t block_bytes = L.bytes();
+  const int block_bytes = L.bytes();
   const int* table = a.tables + (int64_t)(tile.b < a.B ? tile.b : 0) * a.ld_table;
 
-  // ---- unpacking: what a thread takes of a step's tokens
-  // keys: token kt of the step, dwords kq D/32 + k0 .. + C - 1
-  // values: units va and va + 2 of four tokens, words m of group vg, nibbles j0 .. j0 + C - 1
+  // ---- unpacking: a wave takes 16 tokens of a step (which one page holds)
+  // keys: token kt, dwords qq D/32 + k0 .. + C - 1
+  // values: units u0 and u0 + 2 of four tokens, words n16 of group vg; of heads of 64 half the nibbles
   const int n16 = lane & 15, qq = lane >> 4;
-  const int kt = D == 256 ? 16 * (wave & 1) + n16 : 16 * wave + n16, k0 = D == 256 ? 4 * (wave >> 1) : 0;
-  const int vt = D == 256 ? 0 : wave >> 1, va = 8 * vt + 4 * (qq >> 1) + (qq & 1);
-  const int vg = D == 256 ? wave : D == 128 ? wave & 1 : 0, j0 = D == 64 ? 2 * (wave & 1) : 0;
+  const int sub = D == 256 ? wave & 1 : wave, kt = 16 * sub + n16, k0 = D == 256 ? 4 * (wave >> 1) : 0;
+  const int u0 = qq & 1, vg = D == 64 ? 0 : (D == 256 ? 2 * (wave >> 1) : 0) + (qq >> 1);
+  const int k_lane = n16 * (D / 2) + (qq * (D / 32) + k0) * 4, ks_lane = (n16 * G + k0 / 2) * 4;
+  const int v_lane = (u0 * 16 + n16) * (8 * G) + vg * 8, vs_lane = (u0 * G + vg) * 16;
   struct Raw {
     uint32_t k[C], ks[KG], v[4], vs[2][4];
   };
@@ -1011,28 +1039,17 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
   int ids = 0;
   uint64_t gone = 0;
   auto load = [&](int at, int step, Raw& r) {
-    auto block_of = [&](int sub) {
-      return a.cache + ((int64_t)__builtin_amdgcn_readlane(ids, E * at + sub) * a.Hkv + hk) * block_bytes;
-    };
-    {
-      const int sub = D == 256 ? wave & 1 : wave;
-      const uint8_t* block = block_of(sub);
-      const int tl = ((step * TT + 16 * sub) & (a.P - 1)) + n16;
-      const uint8_t* kp = block + tl * (D / 2) + (qq * (D / 32) + k0) * 4;
-      __builtin_memcpy(r.k, __builtin_assume_aligned(kp, C * 4), C * 4);
-      const uint8_t* sp = block + L.k_scales() + (tl * G + k0 / 2) * 4;
-      __builtin_memcpy(r.ks, __builtin_assume_aligned(sp, KG * 4), KG * 4);
-    }
+    const int id = __builtin_amdgcn_readlane(ids, E * at + sub);
+    const bool in = id >= 0 && id < a.pages;  // else a block of no bytes, which reads as zeros
+    const auto block = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(a.cache) + ((int64_t)(in ? id : 0) * a.Hkv + hk) * block_bytes, 0, in ? block_bytes : 0, 0x00020000);
+    const int tl = (step * TT + 16 * sub) & (a.P - 1);
+    fetch<C>(r.k, block, k_lane, tl * (D / 2));
+    fetch<KG>(r.ks, block, ks_lane, L.k_scales() + tl * (G * 4));
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {  // units va and va + 2 of a 32-token half: one 16-token page part each pair of lanes
-      const int sub0 = 2 * vt + (qq >> 1);
-      const int id = __shfl(ids, E * at + sub0, 64);
-      const uint8_t* block = a.cache + ((int64_t)id * a.Hkv + hk) * block_bytes;
-      const int tl = ((step * TT + 16 * sub0) & (a.P - 1)) / 4 + (qq & 1) + 2 * x;
-      const uint8_t* vp = block + L.v_codes() + ((tl * 16 + n16) * G + vg) * 8;
-      __builtin_memcpy(r.v + 2 * x, __builtin_assume_aligned(vp, 8), 8);
-      const uint8_t* wp = block + L.v_scales() + (tl * G + vg) * 16;
-      __builtin_memcpy(r.vs[x], __builtin_assume_aligned(wp, 16), 16);
+    for (int x = 0; x < 2; ++x) {
+      fetch<2>(r.v + 2 * x, block, v_lane, L.v_codes() + tl * (32 * G) + x * (256 * G));
+      fetch<4>(r.vs[x], block, vs_lane, L.v_scales() + tl * (G * 4) + x * (32 * G));
     }
   };
   auto unpack = [&](int at, int step, Raw& r, Tile& t) {
@@ -1044,8 +1061,8 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
       for (int x = 0; x < 2; ++x)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          const int tok = t0 + 4 * (va + 2 * x) + 2 * c;
-          const bool ok = !(bad >> (2 * vt + (qq >> 1)) & 1);
+          const int tok = t0 + 16 * sub + 4 * (u0 + 2 * x) + 2 * c;
+          const bool ok = !(bad >> sub & 1);
           const uint32_t keep = (ok && tok >= lo && tok < hi ? 0xffffu : 0u) | (ok && tok + 1 >= lo && tok + 1 < hi ? 0xffff0000u : 0u);
           r.vs[x][c] &= keep;
           r.vs[x][2 + c] &= keep;
@@ -1056,15 +1073,14 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
     for (int c = 0; c < C; ++c) kd[(2 * (k0 + c) + (qq >> 1)) * 64] = O::key(r.k[c], r.ks[c / 2]);
     const uint32_t s[4] = {r.vs[0][0], r.vs[0][1], r.vs[1][0], r.vs[1][1]};
     const uint32_t z[4] = {r.vs[0][2], r.vs[0][3], r.vs[1][2], r.vs[1][3]};
-    Frag* vd = t.v + (2 * vg * (TT / 16) + 2 * vt + (qq >> 1)) * 64 + (qq & 1) * 32 + n16;
-    if constexpr (D == 64) {
-      if (j0 == 0) {
-        vd[0] = O::template val<0>(r.v, s, z);
-        vd[16] = O::template val<1>(r.v, s, z);
-      } else {
-        vd[(TT / 16) * 64] = O::template val<2>(r.v, s, z);
-        vd[(TT / 16) * 64 + 16] = O::template val<3>(r.v, s, z);
-      }
+    Frag* vd = t.v + (2 * vg * (TT / 16) + sub) * 64 + u0 * 32 + n16;
+    if constexpr (D == 64) {  // nibbles 2 (qq >> 1) and the next, moved to the place of 0 and 1
+      uint32_t u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = r.v[i] >> (16 * (qq >> 1));
+      vd += (qq >> 1) * (TT / 16) * 64;
+      vd[0] = O::template val<0>(u, s, z);
+      vd[16] = O::template val<1>(u, s, z);
     } else {
       vd[0] = O::template val<0>(r.v, s, z);
       vd[16] = O::template val<1>(r.v, s, z);
@@ -1084,8 +1100,8 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            t.vs[vg][4 * (va + 2 * x) + e] = f16_bits_to_f32((uint16_t)(r.vs[x][e >> 1] >> (16 * (e & 1))));
-            t.vl[vg][4 * (va + 2 * x) + e] = f16_bits_to_f32((uint16_t)(r.vs[x][2 + (e >> 1)] >> (16 * (e & 1))));
+            t.vs[vg][16 * sub + 4 * (u0 + 2 * x) + e] = f16_bits_to_f32((uint16_t)(r.vs[x][e >> 1] >> (16 * (e & 1))));
+            t.vl[vg][16 * sub + 4 * (u0 + 2 * x) + e] = f16_bits_to_f32((uint16_t)(r.vs[x][2 + (e >> 1)] >> (16 * (e & 1))));
           }
       }
     }
@@ -1106,60 +1122,71 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
     if (!busy || t0 > pos_max || (a.window > 0 && t0 + TT <= pos_min - a.window + 1)) return;  // nothing of it is seen
     const bool edge = t0 + TT - 1 > pos_min || t0 + TT > hi || (a.window > 0 && t0 <= pos_max - a.window) || bad;
 #pragma unroll
-    for (int u0 = 0; u0 < U; u0 += UB) {
-      float x[UB][16];
+    for (int h0 = 0; h0 < U; h0 += UB) {
+      f32x16 x[UB];
+      if constexpr (kCodes<T>) {
+        x[0] = f32x16{};
 #pragma unroll
-      for (int u = 0; u < UB; ++u) {
-        if constexpr (kCodes<T>) {
+        for (int g = 0; g < G; ++g) {
+          Frag kf[4];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[u][i] = 0.f;
+          for (int k = 0; k < 4; ++k) kf[k] = t.k[(h0 * KS + 4 * g + k) * 64 + lane];
+          __builtin_amdgcn_sched_barrier(0);
+          f32x16 sc = {};
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
-            f32x16 sc;
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+            for (int p = NP - 1; p >= 0; --p) sc = O::mma(kf[k], qf[4 * g + k][p], sc);
 #pragma unroll
-            for (int k = 4 * g; k < 4 * g + 4; ++k) {
-              const Frag kf = t.k[((u0 + u) * KS + k) * 64 + lane];
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 s4 = *reinterpret_cast<const f32x4*>(&t.ks[g][32 * h0 + 8 * q + 4 * h]);
+            const f32x4 l4 = *reinterpret_cast<const f32x4*>(&t.kl[g][32 * h0 + 8 * q + 4 * h]);
 #pragma unroll
-              for (int p = NP - 1; p >= 0; --p) sc = O::mma(kf, qf[k][p], sc);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const f32x4 s4 = *reinterpret_cast<const f32x4*>(&t.ks[g][32 * (u0 + u) + 8 * q + 4 * h]);
-              const f32x4 l4 = *reinterpret_cast<const f32x4*>(&t.kl[g][32 * (u0 + u) + 8 * q + 4 * h]);
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                x[u][4 * q + e] = __builtin_fmaf(s4[e], sc[4 * q + e], __builtin_fmaf(l4[e], qs[g], x[u][4 * q + e]));
-            }
+            for (int e = 0; e < 4; ++e)
+              x[0][4 * q + e] = __builtin_fmaf(s4[e], sc[4 * q + e], __builtin_fmaf(l4[e], qs[g], x[0][4 * q + e]));
           }
-        } else {
-          f32x16 sc;
+        }
+      } else {
+        // every operand is on its way before the first product waits for one
+        Frag kf[UB][KS];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sc[i] = 0.f;
+        for (int u = 0; u < UB; ++u)
 #pragma unroll
-          for (int k = 0; k < KS; ++k) sc = O::mma(t.k[((u0 + u) * KS + k) * 64 + lane], qf[k][0], sc);
+          for (int k = 0; k < KS; ++k) kf[u][k] = t.k[((h0 + u) * KS + k) * 64 + lane];
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) x[u][i] = sc[i];
+        for (int u = 0; u < UB; ++u) {
+          x[u] = f32x16{};
+#pragma unroll
+          for (int k = 0; k < KS; ++k) x[u] = O::mma(kf[u][k], qf[k][0], x[u]);
         }
       }
-      if (edge) {
+      Frag vf[2][DT];
+      auto load_values_of = [&](int i, Frag (&f)[DT]) {  // tokens 16 i .. of the half (or halves)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) f[d] = t.v[(d * (TT / 16) + 2 * h0 + i) * 64 + lane];
+      };
+      __builtin_amdgcn_sched_barrier(0);
+      load_values_of(0, vf[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (edge) {  // the row sees tokens from + 4 h + t0 .. upto + 4 h + t0
+        const int last = pos < hi - 1 ? pos : hi - 1, upto = last - t0 - 4 * h - 32 * h0;
+        const int from = a.window > 0 ? pos - a.window + 1 - t0 - 4 * h - 32 * h0 : -(1 << 30);
 #pragma unroll
         for (int u = 0; u < UB; ++u)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int tok = t0 + 32 * (u0 + u) + 8 * (i >> 2) + 4 * h + (i & 3);
-            const bool see = tok <= pos && tok < hi && (a.window <= 0 || tok > pos - a.window) &&
-                             !(bad >> (2 * (u0 + u) + (i >> 3)) & 1);
-            x[u][i] = see ? x[u][i] : -__builtin_inff();
+            const int at = 32 * u + 8 * (i >> 2) + (i & 3);
+            const bool hide = (at > upto) | (at < from) | ((bad >> (2 * (h0 + u) + (i >> 3)) & 1) != 0);
+            x[u][i] = hide ? -__builtin_inff() : x[u][i];
           }
       }
-      float top = x[0][0] *= rs;
+      float top = x[0][0];
 #pragma unroll
       for (int u = 0; u < UB; ++u)
 #pragma unroll
-        for (int i = u ? 0 : 1; i < 16; ++i) top = fmaxf(top, x[u][i] *= rs);
-      top = pair_max(top);
+        for (int i = u ? 0 : 1; i < 16; ++i) top = top_of(top, x[u][i]);
+      top = pair_max(top) * rs;
       if (__any(top > m + kSlack)) {
         const float to = max_of(m, top);
         const float f = to == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - to);
@@ -1172,41 +1199,43 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
       }
       const float base = m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
-      for (int u = 0; u < UB; ++u)
+      for (int i = 0; i < 2 * UB; ++i) {
+        if (i + 1 < 2 * UB) load_values_of(i + 1, vf[(i + 1) & 1]);
+        const int u = i >> 1, s = i & 1;
+        float p[8];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          float p[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            p[e] = __builtin_amdgcn_exp2f(x[u][8 * s + e] - base);
-            l += p[e];
-          }
-          Frag pf[NP];
-          if constexpr (!kCodes<T>) parts_of(p, pf);
-#pragma unroll
-          for (int g = 0; g < G; ++g) {
-            if constexpr (kCodes<T>) {
-              float w[8];
-#pragma unroll
-              for (int q = 0; q < 2; ++q) {
-                const f32x4 s4 = *reinterpret_cast<const f32x4*>(&t.vs[g][32 * (u0 + u) + 16 * s + 8 * q + 4 * h]);
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(&t.vl[g][32 * (u0 + u) + 16 * s + 8 * q + 4 * h]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  w[4 * q + e] = p[4 * q + e] * s4[e];
-                  ol[g] = __builtin_fmaf(p[4 * q + e], l4[e], ol[g]);
-                }
-              }
-              parts_of(w, pf);
-            }
-#pragma unroll
-            for (int d = 2 * g; d < 2 * g + 2; ++d) {
-              const Frag vf = t.v[(d * (TT / 16) + 2 * (u0 + u) + s) * 64 + lane];
-#pragma unroll
-              for (int q = NP - 1; q >= 0; --q) o[d] = O::mma(vf, pf[q], o[d]);
-            }
-          }
+        for (int e = 0; e < 8; ++e) {
+          p[e] = weight_of<T>(x[u][8 * s + e], rs, base);
+          if constexpr (kCodes<T>) l += p[e];
         }
+        Frag pf[NP];
+        if constexpr (!kCodes<T>) {
+          parts_of(p, pf);
+          l = add_weights(p, pf, l);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          if constexpr (kCodes<T>) {
+            float w[8];
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const f32x4 s4 = *reinterpret_cast<const f32x4*>(&t.vs[g][32 * (h0 + u) + 16 * s + 8 * q + 4 * h]);
+              const f32x4 l4 = *reinterpret_cast<const f32x4*>(&t.vl[g][32 * (h0 + u) + 16 * s + 8 * q + 4 * h]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                w[4 * q + e] = p[4 * q + e] * s4[e];
+                ol[g] = __builtin_fmaf(p[4 * q + e], l4[e], ol[g]);
+              }
+            }
+            parts_of(w, pf);
+          }
+#pragma unroll
+          for (int d = 2 * g; d < 2 * g + 2; ++d)
+#pragma unroll
+            for (int q = NP - 1; q >= 0; --q) o[d] = O::mma(vf[i & 1][d], pf[q], o[d]);
+        }
+      }
     }
   };
 
@@ -1218,7 +1247,6 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
       ids = used ? table[t >> a.shift] : -1;
       const bool bad = ids < 0 || ids >= a.pages;
       gone = __ballot(bad);
-      if (bad) ids = 0;  // in bounds, and not seen
     }
     Raw raw;
     load(0, r0, raw);
