@@ -99,6 +99,14 @@ struct Device {
   }
 };
 
+// A vector over part of a tensor's storage, `offset` in values of its own type.
+at::Tensor part_of(const at::Tensor& whole, at::ScalarType type, int64_t offset, int64_t size) {
+  auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), at::scalarTypeToTypeMeta(type));
+  impl->set_storage_offset(offset);
+  impl->set_sizes_contiguous(at::IntArrayRef(&size, 1));
+  return at::Tensor(std::move(impl));
+}
+
 at::Tensor vector_of(const at::Tensor& t, at::ScalarType type) {
   if (t.scalar_type() == type && t.is_contiguous()) return t;
   return t.to(type).contiguous();
@@ -207,8 +215,12 @@ PyObject* plan_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     REFUSE(T < 0, "tokens must not be negative");
     Device d;
     d.add(ring), d.add(state), d.add(tables), d.add(past), d.add(fresh);
-    at::Tensor slots = d.empty({T}, at::kLong), positions = d.empty({T}, at::kInt), requests = d.empty({T}, at::kInt);
-    at::Tensor starts = d.empty({B + 1}, at::kInt), context = d.empty({B}, at::kInt), next = d.empty({3}, at::kLong);
+    // one allocation: slots and state in int64, then the rest in int32
+    const at::Tensor all = d.empty({T + 3 + T + B + 1}, at::kLong);
+    const int64_t words = 2 * (T + 3);
+    at::Tensor slots = part_of(all, at::kLong, 0, T), next = part_of(all, at::kLong, T, 3);
+    at::Tensor positions = part_of(all, at::kInt, words, T), requests = part_of(all, at::kInt, words + T, T);
+    at::Tensor starts = part_of(all, at::kInt, words + 2 * T, B + 1), context = part_of(all, at::kInt, words + 2 * T + B + 1, B);
     check(entry.plan_step(static_cast<int32_t*>(ring.data_ptr()), ring.numel(), static_cast<int64_t*>(state.data_ptr()),
                           static_cast<int64_t*>(next.data_ptr()), static_cast<int32_t*>(tables.data_ptr()), tables.stride(0),
                           tables.size(1), static_cast<int32_t*>(past.data_ptr()), static_cast<int32_t*>(fresh.data_ptr()), B,

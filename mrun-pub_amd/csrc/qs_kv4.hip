@@ -28,35 +28,9 @@ struct AppendArgs {
   uint8_t* cache;
   int64_t ldk_t, ldk_h, ldv_t, ldv_h, ldq_t, ldq_h;
   int64_t slots_all;  // pages * P
-  int P, D, Hkv, Hq, rot, interleaved;
+  int P, D, Hkv, Hq, rot, interleaved, wide;  // wide: 16 bytes of queries an item
   double mag;
 };
-
-// Four values of a head from d on, turned.
-template <class T>
-__device__ __forceinline__ void turned4(const T* x, int d, int rot, int interleaved, const float2* cs, float (&v)[4]) {
-  load_values<T, 4>(x + d, v);
-  if (d >= rot) return;
-  const int half = rot / 2;
-  if (interleaved) {
-#pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-      const float2 w = cs[(d + e) / 2];
-      const float x1 = v[e], x2 = v[e + 1];
-      v[e] = x1 * w.x - x2 * w.y;
-      v[e + 1] = x2 * w.x + x1 * w.y;
-    }
-  } else {
-    const bool low = d < half;
-    float o[4];
-    load_values<T, 4>(x + (low ? d + half : d - half), o);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 w = cs[(low ? d : d - half) + e];
-      v[e] = low ? v[e] * w.x - o[e] * w.y : v[e] * w.x + o[e] * w.y;
-    }
-  }
-}
 
 // Maximum over the 16 lanes of a row, in every lane of it.
 __device__ __forceinline__ float row_max(float v) {
@@ -92,45 +66,112 @@ __device__ __forceinline__ uint32_t code4(const float (&x)[4], _Float16& s16, _F
   return s > 0.f ? c : 0u;
 }
 
+// Four values of a head from d on, and with the halves' layout their partners.
+template <class T>
+struct Quad {
+  float v[4], o[4];
+  __device__ __forceinline__ void load(const T* x, int d, int rot, int interleaved) {
+    load_values<T, 4>(x + d, v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = 0.f;
+    if (d < rot && !interleaved) load_values<T, 4>(x + (d < rot / 2 ? d + rot / 2 : d - rot / 2), o);
+  }
+  __device__ __forceinline__ void turn(int d, int rot, int interleaved, const float2* cs) {
+    if (d >= rot) return;
+    // partners and factors by selection: the interleaved layout's partner is the value next to it
+    const bool low = d < rot / 2;
+    const float2* w = cs + (interleaved ? d / 2 : low ? d : d - rot / 2);
+    float r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = w[interleaved ? e / 2 : e];
+      const float other = interleaved ? v[e ^ 1] : o[e];
+      const bool first = interleaved ? !(e & 1) : low;
+      r[e] = first ? v[e] * f.x - other * f.y : v[e] * f.x + other * f.y;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = r[e];
+  }
+};
+
 template <class T>
 __global__ __launch_bounds__(256) void k_kv4_append(AppendArgs a) {
+  using Item = TurnItem<T>;
   __shared__ float2 cs[128];
   const int64_t t = blockIdx.x;
-  if (a.rot) {
-    for (int i = threadIdx.x; i < a.rot / 2; i += 256) cs[i] = rotary_cos_sin(a.pos[t], a.freq[i], a.mag);
-    __syncthreads();
-  }
-  const int quads = a.D / 4;
+  const Kv4Layout L(a.P, a.D);
+  const int64_t slot = a.slots[t];
   const T* q = static_cast<const T*>(a.q) + t * a.ldq_t;
   T* qo = static_cast<T*>(a.q_out) + t * a.Hq * a.D;
-  for (int i = threadIdx.x; i < a.Hq * quads; i += 256) {
-    const int h = i / quads, d = (i - h * quads) * 4;
-    float v[4];
-    turned4<T>(q + h * a.ldq_h, d, a.rot, a.interleaved, cs, v);
-    store_values<T, 4>(qo + h * a.D + d, v);
+  // queries: items of 16 bytes, or of four values
+  const int turned = a.wide ? Item::turned(a.rot, a.interleaved) : 0;
+  const int per_head = a.wide ? turned + (a.D - a.rot) / Item::V : a.D / 4;
+  const int items = a.Hq * per_head;
+  // keys, then values: 16 lanes a (head, group); a whole row of lanes is in or out
+  const int groups = a.Hkv * L.G, m = threadIdx.x & 15;
+  auto group_of = [&](int i, int& h, int& d) {
+    const int hg = i < groups ? i : i - groups;
+    h = hg / L.G;
+    d = (hg - h * L.G) * kKv4Group + 4 * m;
+  };
+  auto load_quad = [&](int i, int h, int d, Quad<T>& x) {
+    if (i < groups)
+      x.load(static_cast<const T*>(a.k) + t * a.ldk_t + h * a.ldk_h, d, a.rot, a.interleaved);
+    else
+      load_values<T, 4>(static_cast<const T*>(a.v) + t * a.ldv_t + h * a.ldv_h + d, x.v);
+  };
+  // the first of each is under way while the angles are computed
+  Item item;
+  Quad<T> quad;
+  int h, d, qh = 0;
+  const bool wide = a.wide;
+  if (wide && threadIdx.x < items) {
+    qh = threadIdx.x / per_head;
+    item.load(q + qh * a.ldq_h, threadIdx.x - qh * per_head, turned, a.rot, a.interleaved);
   }
-  const int64_t slot = a.slots[t];
-  if (slot < 0 || slot >= a.slots_all) return;
-  const Kv4Layout L(a.P, a.D);
+  const bool in = slot >= 0 && slot < a.slots_all;
+  int i = threadIdx.x >> 4;
+  group_of(i, h, d);
+  if (in && i < 2 * groups) load_quad(i, h, d, quad);
+  if (a.rot) {
+    for (int j = threadIdx.x; j < a.rot / 2; j += 256) cs[j] = rotary_cos_sin(a.pos[t], a.freq[j], a.mag);
+    __syncthreads();
+  }
+  if (wide) {
+    for (int j = threadIdx.x; j < items; j += 256) {
+      if (j >= 256) {
+        qh = j / per_head;
+        item.load(q + qh * a.ldq_h, j - qh * per_head, turned, a.rot, a.interleaved);
+      }
+      item.store(qo + qh * a.D, j - qh * per_head, turned, a.rot, a.interleaved, cs);
+    }
+  } else {
+    for (int j = threadIdx.x; j < items; j += 256) {
+      const int qd = (j % per_head) * 4;
+      Quad<T> x;
+      qh = j / per_head;
+      x.load(q + qh * a.ldq_h, qd, a.rot, a.interleaved);
+      x.turn(qd, a.rot, a.interleaved, cs);
+      store_values<T, 4>(qo + qh * a.D + qd, x.v);
+    }
+  }
+  if (!in) return;
   const int64_t page = slot / a.P;
   const int row = (int)(slot - page * a.P);
-  // 16 lanes a (key or value, head, group); a whole row of lanes is in or out
-  const int groups = a.Hkv * L.G;
-  for (int i = threadIdx.x >> 4; i < 2 * groups; i += 16) {
+  for (; i < 2 * groups; i += 16) {
+    if (i >= 16) {
+      group_of(i, h, d);
+      load_quad(i, h, d, quad);
+    }
     const bool key = i < groups;
-    const int hg = key ? i : i - groups;
-    const int h = hg / L.G, g = hg - h * L.G, m = threadIdx.x & 15;
-    const int d = g * kKv4Group + 4 * m;
-    float v[4];
     if (key) {
-      turned4<T>(static_cast<const T*>(a.k) + t * a.ldk_t + h * a.ldk_h, d, a.rot, a.interleaved, cs, v);
+      quad.turn(d, a.rot, a.interleaved, cs);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = to_f32(from_f32<T>(v[e]));
-    } else {
-      load_values<T, 4>(static_cast<const T*>(a.v) + t * a.ldv_t + h * a.ldv_h + d, v);
+      for (int e = 0; e < 4; ++e) quad.v[e] = to_f32(from_f32<T>(quad.v[e]));
     }
     _Float16 s, lo;
-    const uint32_t c = code4(v, s, lo);
+    const uint32_t c = code4(quad.v, s, lo);
+    const int g = d / kKv4Group;
     uint8_t* block = a.cache + (page * a.Hkv + h) * (int64_t)L.bytes();
     if (key) {
       // a nibble in each byte: the even lane's low ones, the odd lane's high ones
@@ -220,7 +261,10 @@ extern "C" int qs_kv4_append(const void* k, int64_t ldk_t, int64_t ldk_h, const 
       !aligned(cache, 16))
     return fail(QS_ERR_INVALID, "kv4_append: heads are aligned to four values");
   AppendArgs a{k, v, q, q_out, slots, positions, freq, cache, ldk_t, ldk_h, ldv_t, ldv_h, ldq_t, ldq_h,
-               pages * page_size, (int)page_size, D, Hkv, Hq, rot, interleaved, magnitude};
+               pages * page_size, (int)page_size, D, Hkv, Hq, rot, interleaved, 0, magnitude};
+  const int per16 = 16 / size;
+  a.wide = Hq > 0 && aligned(q, 16) && aligned(q_out, 16) && ldq_t % per16 == 0 && ldq_h % per16 == 0 &&
+           (size == 4 ? TurnItem<float>::fits(D, rot, interleaved) : TurnItem<__bf16>::fits(D, rot, interleaved));
   const dim3 grid((unsigned)T), block(256);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (dtype == QS_F32)

@@ -17,8 +17,8 @@
 namespace qs {
 namespace {
 
-constexpr int kPlanThreads = 256;
-constexpr int kPlanTokens = 1024;  // of a block
+constexpr int kPlanThreads = 512;
+constexpr int kPlanTokens = 512;  // of a block
 
 struct PlanArgs {
   const int* ring;
@@ -69,8 +69,10 @@ __device__ __forceinline__ Scan block_scan(int64_t v, int64_t* part) {
   return r;
 }
 
-__device__ __forceinline__ int64_t ring_page(const PlanArgs& p, int64_t head, int64_t avail, int64_t rank) {
-  return rank < avail ? p.ring[(uint64_t)(head + rank) % (uint64_t)p.ring_size] : -1;
+// Ring entry `at` places after place `from` (both below the ring's size).
+__device__ __forceinline__ int64_t ring_at(int64_t from, int64_t at, int64_t size) {
+  const int64_t i = from + at;
+  return i < size ? i : i - size;
 }
 
 __global__ __launch_bounds__(kPlanThreads) void k_plan_step(PlanArgs p) {
@@ -79,6 +81,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan_step(PlanArgs p) {
   __shared__ int s_past[kPlanThreads];
   const int64_t head = p.state[0], tail = p.state[1];
   const int64_t avail = tail > head ? (tail - head < p.ring_size ? tail - head : p.ring_size) : 0;
+  const int64_t from = (int64_t)((uint64_t)head % (uint64_t)p.ring_size);
   const int64_t t0 = (int64_t)blockIdx.x * kPlanTokens;
   const int64_t t1 = t0 + kPlanTokens < p.T ? t0 + kPlanTokens : p.T;
   int64_t tokens = 0, pages = 0;  // of the requests before this chunk
@@ -125,7 +128,8 @@ __global__ __launch_bounds__(kPlanThreads) void k_plan_step(PlanArgs p) {
         if (col < own) {
           page = *entry;
         } else {
-          page = ring_page(p, head, avail, s_rank[at] + col);
+          const int64_t rank = s_rank[at] + col;
+          if (rank < avail) page = p.ring[ring_at(from, rank, p.ring_size)];
           if ((pos & (p.P - 1)) == 0) *entry = (int)page;
         }
       }
@@ -164,7 +168,7 @@ struct ReleaseArgs {
   int B, P, shift;
 };
 
-// One block: the finished requests in turn, 256 table columns at a time.  Only pages come back: a
+// One block: the finished requests in turn, 512 table columns at a time.  Only pages come back: a
 // table entry of -1 (no page was left for it) takes no place in the ring.
 __global__ __launch_bounds__(kPlanThreads) void k_release_pages(ReleaseArgs p) {
   __shared__ int64_t part[kPlanThreads / 64];

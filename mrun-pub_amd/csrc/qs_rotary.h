@@ -1,7 +1,7 @@
 // Rotary angles, shared by the kernels that turn activations.
 #pragma once
 
-#include "qs_common.h"
+#include "qs_values.h"
 
 namespace qs {
 
@@ -39,5 +39,46 @@ __device__ __forceinline__ float2 rotary_cos_sin(int pos, double freq, double ma
   const double sn = quarter >= 2 ? -sw : sw;
   return {(float)(cs * mag), (float)(sn * mag)};
 }
+
+// Sixteen bytes of a head's turned values, with the halves' layout their partners' sixteen, or of the
+// values behind them: item c of `turned` + (D - rot) / V.  Heads aligned to 16 bytes, sizes that divide.
+template <class T>
+struct TurnItem {
+  static constexpr int V = 16 / sizeof(T);
+  float a[V], b[V];
+  static __device__ __forceinline__ int turned(int rot, int interleaved) { return interleaved ? rot / V : rot / 2 / V; }
+  static __host__ __device__ __forceinline__ bool fits(int D, int rot, int interleaved) {
+    return D % V == 0 && rot % (interleaved ? V : 2 * V) == 0;
+  }
+  __device__ __forceinline__ void load(const T* x, int c, int turned, int rot, int interleaved) {
+    load_values<T, V>(x + (c < turned ? c * V : rot + (c - turned) * V), a);
+    if (c < turned && !interleaved) load_values<T, V>(x + rot / 2 + c * V, b);
+  }
+  // cs: cos and sin of the token's pairs
+  __device__ __forceinline__ void store(T* y, int c, int turned, int rot, int interleaved, const float2* cs) {
+    if (c >= turned) {
+      store_values<T, V>(y + rot + (c - turned) * V, a);
+    } else if (interleaved) {
+      const float2* w = cs + c * (V / 2);
+#pragma unroll
+      for (int e = 0; e < V; e += 2) {
+        const float x1 = a[e], x2 = a[e + 1];
+        a[e] = x1 * w[e / 2].x - x2 * w[e / 2].y;
+        a[e + 1] = x2 * w[e / 2].x + x1 * w[e / 2].y;
+      }
+      store_values<T, V>(y + c * V, a);
+    } else {
+      const float2* w = cs + c * V;
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float x1 = a[e], x2 = b[e];
+        a[e] = x1 * w[e].x - x2 * w[e].y;
+        b[e] = x2 * w[e].x + x1 * w[e].y;
+      }
+      store_values<T, V>(y + c * V, a);
+      store_values<T, V>(y + rot / 2 + c * V, b);
+    }
+  }
+};
 
 }  // namespace qs

@@ -38,49 +38,33 @@ __device__ __forceinline__ void block_angles(const RotaryArgs& a, int64_t t0, fl
 
 template <class T>
 __global__ __launch_bounds__(256) void k_rotary_v(RotaryArgs a) {
-  constexpr int V = 16 / sizeof(T);
+  using Item = TurnItem<T>;
   extern __shared__ float2 cs[];
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
-  const int half = a.rot / 2;
-  const int turned = a.interleaved ? a.rot / V : half / V;  // items of a head that turn
-  const int per_head = turned + (a.D - a.rot) / V;
+  const int turned = Item::turned(a.rot, a.interleaved);  // items of a head that turn
+  const int per_head = turned + (a.D - a.rot) / Item::V;
   const int per_token = per_head * a.H;
-  block_angles(a, t0, cs);
   const int64_t left = a.T - t0;
   const int items = per_token * (int)(left < a.tokens ? left : a.tokens);
+  auto at = [&](int i, int& t, int& c, int& h) {
+    t = i / per_token;
+    const int rest = i - t * per_token;
+    h = rest / per_head;
+    c = rest - h * per_head;
+  };
+  Item item;  // the first is under way while the angles are computed
+  int t, c, h;
+  if (threadIdx.x < items) {
+    at(threadIdx.x, t, c, h);
+    item.load(static_cast<const T*>(a.x) + (t0 + t) * a.ldx_t + h * a.ldx_h, c, turned, a.rot, a.interleaved);
+  }
+  block_angles(a, t0, cs);
   for (int i = threadIdx.x; i < items; i += 256) {
-    const int t = i / per_token, rest = i - t * per_token;
-    const int h = rest / per_head, c = rest - h * per_head;
-    const T* x = static_cast<const T*>(a.x) + (t0 + t) * a.ldx_t + h * a.ldx_h;
-    T* y = static_cast<T*>(a.y) + (t0 + t) * a.ldy_t + h * a.ldy_h;
-    if (c >= turned) {
-      const int d = a.rot + (c - turned) * V;
-      *reinterpret_cast<i32x4*>(y + d) = *reinterpret_cast<const i32x4*>(x + d);
-    } else if (a.interleaved) {
-      const float2* w = cs + t * half + c * (V / 2);
-      float v[V];
-      load_values<T, V>(x + c * V, v);
-#pragma unroll
-      for (int e = 0; e < V; e += 2) {
-        const float x1 = v[e], x2 = v[e + 1];
-        v[e] = x1 * w[e / 2].x - x2 * w[e / 2].y;
-        v[e + 1] = x2 * w[e / 2].x + x1 * w[e / 2].y;
-      }
-      store_values<T, V>(y + c * V, v);
-    } else {
-      const float2* w = cs + t * half + c * V;
-      float v1[V], v2[V];
-      load_values<T, V>(x + c * V, v1);
-      load_values<T, V>(x + half + c * V, v2);
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float x1 = v1[e], x2 = v2[e];
-        v1[e] = x1 * w[e].x - x2 * w[e].y;
-        v2[e] = x2 * w[e].x + x1 * w[e].y;
-      }
-      store_values<T, V>(y + c * V, v1);
-      store_values<T, V>(y + half + c * V, v2);
+    if (i >= 256) {
+      at(i, t, c, h);
+      item.load(static_cast<const T*>(a.x) + (t0 + t) * a.ldx_t + h * a.ldx_h, c, turned, a.rot, a.interleaved);
     }
+    item.store(static_cast<T*>(a.y) + (t0 + t) * a.ldy_t + h * a.ldy_h, c, turned, a.rot, a.interleaved, cs + t * (a.rot / 2));
   }
 }
 
@@ -114,7 +98,7 @@ __global__ __launch_bounds__(256) void k_rotary_1(RotaryArgs a) {
 template <class T>
 int launch_rotary(RotaryArgs a, hipStream_t s) {
   constexpr int V = 16 / sizeof(T);
-  const bool wide = a.D % V == 0 && a.rot % (a.interleaved ? V : 2 * V) == 0 && aligned(a.x, 16) && aligned(a.y, 16) &&
+  const bool wide = TurnItem<T>::fits(a.D, a.rot, a.interleaved) && aligned(a.x, 16) && aligned(a.y, 16) &&
                     a.ldx_t % V == 0 && a.ldx_h % V == 0 && a.ldy_t % V == 0 && a.ldy_h % V == 0;
   const int64_t per_token = (int64_t)a.H * (wide ? (a.interleaved ? a.D / V : a.D / V - a.rot / 2 / V)
                                                  : a.D - a.rot / 2);
