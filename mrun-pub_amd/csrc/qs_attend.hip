@@ -46,20 +46,25 @@ struct AttendArgs {
 // A byte 0..15 read as an e4m3 number is byte * 2^-9 (subnormals below 8, one binade above), so one
 // conversion with scale 2^9 gives two codes as 16-bit floats.
 //
-// 16-bit activations multiply fp16: cache values are code * s + lo in fp16 (one rounding, 2^-11),
+// bf16 activations multiply fp16: cache values are code * s + lo in fp16 (one rounding, 2^-11),
 // queries are exact, since a row of bf16 is first divided by a power of two that takes its largest
 // value below 1 (8 bits fit fp16's 11 down to 2^-17 of that), weights are fp16.
 //
-// fp32 activations are sums of three bf16 numbers (8 bits each, all of fp32's 24) and multiply the
-// codes, which bf16 holds exactly: q.k = s (q.code) + lo sum(q) a group, and for the output the
-// weights are p s, with p lo summed beside.  Three instructions of the 16-bit rate in place of the
-// fp32 instruction's sixteenfold time.
+// fp16 and fp32 activations, whose own rounding is no coarser than that, multiply the codes, which
+// both 16-bit types hold exactly: q.k = s (q.code) + lo sum(q) a group, and for the output the
+// weights are p s, with p lo summed beside.  fp16 queries are operands as they are, fp32 ones sums of
+// three bf16 numbers (8 bits each, all of fp32's 24); p s is a sum of two or three bf16 numbers.
+// Three instructions of the 16-bit rate replace the fp32 instruction's sixteenfold time.
 constexpr uint32_t kNibbles = 0x0f0f0f0fu;
 
 template <class T>
-constexpr bool kCodes = sizeof(T) == 4;
+constexpr int kKind = __is_same(T, __bf16) ? 0 : sizeof(T) == 2 ? 1 : 2;
 template <class T>
-constexpr int kParts = kCodes<T> ? 3 : 1;
+constexpr bool kCodes = kKind<T> != 0;
+template <class T>
+constexpr int kQueryParts = kKind<T> == 2 ? 3 : 1;
+template <class T>
+constexpr int kWeightParts = kKind<T> + 1;
 
 template <bool HI>
 __device__ __forceinline__ f16x2 f16_codes(uint32_t w) {
@@ -70,82 +75,88 @@ __device__ __forceinline__ bf16x2 bf16_codes(uint32_t w) {
   return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)w, 512.f, HI);
 }
 
+__device__ __forceinline__ f32x4 mma(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mma(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// The eight codes of a key's dword.
+__device__ __forceinline__ void codes_of(uint32_t w, f16x8& f) {
+  const uint32_t a = w & kNibbles, b = w >> 4 & kNibbles;
+  const f16x2 v0 = f16_codes<false>(a), v1 = f16_codes<true>(a), v2 = f16_codes<false>(b), v3 = f16_codes<true>(b);
+  f = f16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+}
+__device__ __forceinline__ void codes_of(uint32_t w, bf16x8& f) {
+  const uint32_t a = w & kNibbles, b = w >> 4 & kNibbles;
+  const bf16x2 v0 = bf16_codes<false>(a), v1 = bf16_codes<true>(a), v2 = bf16_codes<false>(b), v3 = bf16_codes<true>(b);
+  f = bf16x8{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+}
+
 template <class T>
 struct Ops {
-  typedef f16x8 Frag;
-  static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-  }
+  typedef std::conditional_t<kKind<T> == 2, bf16x8, f16x8> KFrag;  // of keys and queries
+  typedef std::conditional_t<kCodes<T>, bf16x8, f16x8> VFrag;      // of values and weights
   // One dword of a token's key, and its (s, lo).
-  static __device__ __forceinline__ Frag key(uint32_t w, uint32_t sl) {
-    const f16x2 h = __builtin_bit_cast(f16x2, sl);
-    const f16x2 s = {h[0], h[0]}, lo = {h[1], h[1]};
-    const uint32_t a = w & kNibbles, b = w >> 4 & kNibbles;
-    const f16x2 v0 = __builtin_elementwise_fma(f16_codes<false>(a), s, lo);
-    const f16x2 v1 = __builtin_elementwise_fma(f16_codes<true>(a), s, lo);
-    const f16x2 v2 = __builtin_elementwise_fma(f16_codes<false>(b), s, lo);
-    const f16x2 v3 = __builtin_elementwise_fma(f16_codes<true>(b), s, lo);
-    return Frag{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
+  static __device__ __forceinline__ KFrag key(uint32_t w, uint32_t sl) {
+    KFrag f;
+    codes_of(w, f);
+    if constexpr (!kCodes<T>) {
+      const f16x2 h = __builtin_bit_cast(f16x2, sl);
+      const f16x2 s = {h[0], h[0]}, lo = {h[1], h[1]};
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const f16x2 v = __builtin_elementwise_fma(f16x2{f[i], f[i + 1]}, s, lo);
+        f[i] = v[0];
+        f[i + 1] = v[1];
+      }
+    }
+    return f;
   }
   // Values 4 m + J of eight tokens: u holds the bytes of token pairs, s and lo the pairs' own.
   template <int J>
-  static __device__ __forceinline__ Frag val(const uint32_t (&u)[4], const uint32_t (&s)[4], const uint32_t (&lo)[4]) {
-    Frag f;
+  static __device__ __forceinline__ VFrag val(const uint32_t (&u)[4], const uint32_t (&s)[4], const uint32_t (&lo)[4]) {
+    VFrag f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const uint32_t w = (J & 1 ? u[i] >> 4 : u[i]) & kNibbles;
-      const f16x2 v = __builtin_elementwise_fma(f16_codes<(J >> 1) != 0>(w), __builtin_bit_cast(f16x2, s[i]),
-                                                __builtin_bit_cast(f16x2, lo[i]));
-      f[2 * i] = v[0];
-      f[2 * i + 1] = v[1];
+      if constexpr (kCodes<T>) {
+        const bf16x2 v = bf16_codes<(J >> 1) != 0>(w);
+        f[2 * i] = v[0];
+        f[2 * i + 1] = v[1];
+      } else {
+        const f16x2 v = __builtin_elementwise_fma(f16_codes<(J >> 1) != 0>(w), __builtin_bit_cast(f16x2, s[i]),
+                                                  __builtin_bit_cast(f16x2, lo[i]));
+        f[2 * i] = v[0];
+        f[2 * i + 1] = v[1];
+      }
     }
     return f;
   }
 };
 
-template <>
-struct Ops<float> {
-  typedef bf16x8 Frag;
-  static __device__ __forceinline__ f32x4 mma(Frag a, Frag b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x16 mma(Frag a, Frag b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ Frag key(uint32_t w, uint32_t) {
-    const uint32_t a = w & kNibbles, b = w >> 4 & kNibbles;
-    const bf16x2 v0 = bf16_codes<false>(a), v1 = bf16_codes<true>(a), v2 = bf16_codes<false>(b), v3 = bf16_codes<true>(b);
-    return Frag{v0[0], v0[1], v1[0], v1[1], v2[0], v2[1], v3[0], v3[1]};
-  }
-  template <int J>
-  static __device__ __forceinline__ Frag val(const uint32_t (&u)[4], const uint32_t (&)[4], const uint32_t (&)[4]) {
-    Frag f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t w = (J & 1 ? u[i] >> 4 : u[i]) & kNibbles;
-      const bf16x2 v = bf16_codes<(J >> 1) != 0>(w);
-      f[2 * i] = v[0];
-      f[2 * i + 1] = v[1];
-    }
-    return f;
-  }
-};
-
-// Eight fp32 values as operands: rounded to fp16, or as three bf16 parts.
+// Eight fp32 values as operands: rounded to fp16, or as two or three bf16 parts.
 __device__ __forceinline__ void parts_of(const float (&v)[8], f16x8 (&p)[1]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) p[0][i] = static_cast<_Float16>(v[i]);
 }
-__device__ __forceinline__ void parts_of(const float (&v)[8], bf16x8 (&p)[3]) {
+template <int N>
+__device__ __forceinline__ void parts_of(const float (&v)[8], bf16x8 (&p)[N]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    p[0][i] = static_cast<__bf16>(v[i]);
-    const float r = v[i] - static_cast<float>(p[0][i]);
-    p[1][i] = static_cast<__bf16>(r);
-    p[2][i] = static_cast<__bf16>(r - static_cast<float>(p[1][i]));
+    float r = v[i];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      p[k][i] = static_cast<__bf16>(r);
+      r -= static_cast<float>(p[k][i]);
+    }
   }
 }
 
@@ -397,6 +408,8 @@ __device__ __forceinline__ Work pick_work(const AttendArgs& a, float* s_sum, Wor
   const unsigned x = blockIdx.x, y = x / (unsigned)a.Hkv;  // heads side by side: each to its own XCD's cache
   Work t = a.blocks > 0 ? pick_part<R, STEP, THREADS>(a, (int)y, s_sum, s_work) : pick_tile<R>(a, y);
   t.hk = (int)(x - y * (unsigned)a.Hkv);
+  t.q0 = __builtin_amdgcn_readfirstlane((int)t.q0);  // both below 2^31
+  t.first = __builtin_amdgcn_readfirstlane((int)t.first);
   t.b = __builtin_amdgcn_readfirstlane(t.b);
   t.n = __builtin_amdgcn_readfirstlane(t.n);
   t.ctx = __builtin_amdgcn_readfirstlane(t.ctx);
@@ -429,7 +442,7 @@ struct QueryRow {
   }
   // Returns what the row's scores have to be multiplied by; sums: this lane's part of its groups' sums.
   template <int G, class Frag>
-  __device__ __forceinline__ float operands(float scale_log2, Frag (&qf)[KS][kParts<T>], float (&sums)[G]) {
+  __device__ __forceinline__ float operands(float scale_log2, Frag (&qf)[KS][kQueryParts<T>], float (&sums)[G]) {
     int e2 = 0;
     if constexpr (__is_same(T, __bf16)) {
       float top = 0.f;
@@ -512,33 +525,37 @@ __device__ __forceinline__ bool last_part(const AttendArgs& a, const Work& w, in
 // ahead: registers hold the next step's codes too, which hides a load's time where few waves run; the
 // other form leaves room for twice the waves where their number does that, in blocks of half the
 // size, which share out ragged requests more evenly.
-constexpr bool few_wide(bool codes, int D, int rt) { return D * rt >= (codes ? 256 : 512); }
-constexpr int few_waves(bool codes, int D, int rt, bool ahead) {  // a SIMD, as the registers allow
-  return few_wide(codes, D, rt) ? 1 : !ahead && D * rt * (codes ? 3 : 1) <= 192 ? 4 : 2;
+constexpr bool few_wide(int kind, int D, int rt) { return D * rt >= (kind == 2 ? 256 : 512); }
+constexpr int few_waves(int kind, int D, int rt, bool ahead) {  // a SIMD, as the registers allow
+  if (few_wide(kind, D, rt)) return 1;
+  return ahead ? 2 : D * rt <= 64 || (kind == 0 && D * rt <= 128) ? 4 : kind == 1 && D * rt <= 128 ? 3 : 2;
 }
-constexpr int few_block(bool codes, int D, int rt, bool ahead) {  // waves of a block
-  return few_wide(codes, D, rt) || !ahead ? 4 : 8;
+constexpr int few_block(int kind, int D, int rt, bool ahead) {  // waves of a block
+  return few_wide(kind, D, rt) || !ahead ? 4 : 8;
 }
-constexpr int few_fill(bool codes, int D, int rt, bool ahead) {  // blocks that run at once
-  return 1024 * few_waves(codes, D, rt, ahead) / few_block(codes, D, rt, ahead);
+constexpr int few_fill(int kind, int D, int rt, bool ahead) {  // blocks that run at once
+  return 1024 * few_waves(kind, D, rt, ahead) / few_block(kind, D, rt, ahead);
 }
 // Where both forms exist, `few steps` takes the first.
-constexpr bool few_ahead(bool codes, int D, int rt, bool few_steps) {
-  if (few_wide(codes, D, rt) || D == 256) return false;
-  return few_steps || few_waves(codes, D, rt, false) == few_waves(codes, D, rt, true);
+constexpr bool few_ahead(int kind, int D, int rt, bool few_steps) {
+  if (few_wide(kind, D, rt) || D == 256 || (kind == 1 && D * rt == 256)) return false;
+  return few_steps || few_waves(kind, D, rt, false) == few_waves(kind, D, rt, true);
 }
+// Whether registers hold two tiles of 16 rows.
+constexpr bool few_pairs(int kind, int D) { return kind == 0 || D < 256; }
 constexpr int kFewLeast = 16, kFewWhole = 32;    // steps of a part at least, steps that stay whole
 constexpr int kRowsLeast = 4, kRowsWhole = 8, kRowsFill = 512;
 
 template <class T, int D, int RT, bool AHEAD>
-__global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_waves(kCodes<T>, D, RT, AHEAD))) void k_attend_few(
+__global__ __launch_bounds__((64 * few_block(kKind<T>, D, RT, AHEAD)), (few_waves(kKind<T>, D, RT, AHEAD))) void k_attend_few(
     const int* starts, const int* context, int tokens, int requests, int Hkv, int grp, int reach, int window, int blocks, AttendArgs a) {
   a.starts = starts, a.context = context, a.T = tokens, a.B = requests, a.Hkv = Hkv, a.grp = grp, a.reach = reach;
   a.window = window, a.blocks = blocks;
-  constexpr int NW = few_block(kCodes<T>, D, RT, AHEAD);
+  constexpr int NW = few_block(kKind<T>, D, RT, AHEAD);
   using O = Ops<T>;
-  typedef typename O::Frag Frag;
-  constexpr int G = D / kKv4Group, KS = D / 32, R = 16 * RT, W = 2 * G, NP = kParts<T>;
+  typedef typename O::KFrag KFrag;
+  typedef typename O::VFrag VFrag;
+  constexpr int G = D / kKv4Group, KS = D / 32, R = 16 * RT, W = 2 * G, NQ = kQueryParts<T>, NP = kWeightParts<T>;
   constexpr int KW = kCodes<T> ? 4 * G : G;  // dwords of key scales: the scores' four tokens, or the operand's own
   __shared__ float s_o[NW][16][D + 4];
   __shared__ float2 s_ml[NW][16];
@@ -610,7 +627,7 @@ __global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_wav
   };
 
   // queries: the lane's row, values d = 32 i + 8 qq + (0..7), under way while the pages arrive
-  Frag qf[RT][KS][NP];
+  KFrag qf[RT][KS][NQ];
   float rs[RT], qs[RT][G];
   int pos[RT];
   QueryRow<T, KS, 32> raw_q[RT];
@@ -690,11 +707,11 @@ __global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_wav
           for (int rt = 0; rt < RT; ++rt) sc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 2 * g; k < 2 * g + 2; ++k) {
-            const Frag kf = O::key(rk.k[h][k], 0);
+            const KFrag kf = O::key(rk.k[h][k], 0);
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-              for (int p = NP - 1; p >= 0; --p) sc[rt] = O::mma(kf, qf[rt][k][p], sc[rt]);
+              for (int p = NQ - 1; p >= 0; --p) sc[rt] = mma(kf, qf[rt][k][p], sc[rt]);
           }
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
@@ -711,9 +728,9 @@ __global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_wav
         for (int rt = 0; rt < RT; ++rt) sc[rt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-          const Frag kf = O::key(rk.k[h][k], rk.s[h][k / 2]);
+          const KFrag kf = O::key(rk.k[h][k], rk.s[h][k / 2]);
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) sc[rt] = O::mma(kf, qf[rt][k][0], sc[rt]);
+          for (int rt = 0; rt < RT; ++rt) sc[rt] = mma(kf, qf[rt][k][0], sc[rt]);
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
@@ -722,7 +739,7 @@ __global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_wav
       }
     }
     float p[RT][8];
-    Frag pf[RT][NP];
+    VFrag pf[RT][NP];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (edge) {
@@ -731,7 +748,7 @@ __global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_wav
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int at = 16 * (e >> 2) + (e & 3);
-          x[rt][e] = (at > upto) | (at < from) ? -__builtin_inff() : x[rt][e];
+          x[rt][e] = ((at > upto) | (at < from)) ? -__builtin_inff() : x[rt][e];
         }
         if (bad)
 #pragma unroll
@@ -791,11 +808,11 @@ __global__ __launch_bounds__((64 * few_block(kCodes<T>, D, RT, AHEAD)), (few_wav
           parts_of(w, pf[rt]);
         }
       }
-      auto product = [&](const Frag& vf, int j) {
+      auto product = [&](const VFrag& vf, int j) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int q = NP - 1; q >= 0; --q) o[rt][g][j] = O::mma(vf, pf[rt][q], o[rt][g][j]);
+          for (int q = NP - 1; q >= 0; --q) o[rt][g][j] = mma(vf, pf[rt][q], o[rt][g][j]);
       };
       product(O::template val<0>(u, s, z), 0);
       product(O::template val<1>(u, s, z), 1);
@@ -966,21 +983,22 @@ template <class T, int D>
 struct RowsTile {
   static constexpr int TT = D == 256 ? 32 : 64, U = TT / 32, G = D / kKv4Group;
   static constexpr int kChunks = TT * D / 8;  // of 16 bytes, for keys and for values
-  typedef typename Ops<T>::Frag Frag;
-  Frag k[kChunks], v[kChunks];
+  typename Ops<T>::KFrag k[kChunks];
+  typename Ops<T>::VFrag v[kChunks];
   float ks[kCodes<T> ? G : 1][kCodes<T> ? TT : 1], kl[kCodes<T> ? G : 1][kCodes<T> ? TT : 1];
   float vs[kCodes<T> ? G : 1][kCodes<T> ? TT : 1], vl[kCodes<T> ? G : 1][kCodes<T> ? TT : 1];
 };
 
 template <class T, int D>
-__global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) void k_attend_rows(
+__global__ __launch_bounds__(256, D == 256 || (kKind<T> == 2 && D == 128) ? 1 : 2) void k_attend_rows(
     const int* starts, const int* context, int tokens, int requests, int Hkv, int grp, int reach, int window, int blocks, AttendArgs a) {
   a.starts = starts, a.context = context, a.T = tokens, a.B = requests, a.Hkv = Hkv, a.grp = grp, a.reach = reach;
   a.window = window, a.blocks = blocks;
   using O = Ops<T>;
-  typedef typename O::Frag Frag;
+  typedef typename O::KFrag KFrag;
+  typedef typename O::VFrag VFrag;
   typedef RowsTile<T, D> Tile;
-  constexpr int G = D / kKv4Group, KS = D / 16, DT = D / 32, NP = kParts<T>, TT = Tile::TT, U = Tile::U, R = 128;
+  constexpr int G = D / kKv4Group, KS = D / 16, DT = D / 32, NQ = kQueryParts<T>, NP = kWeightParts<T>, TT = Tile::TT, U = Tile::U, R = 128;
   constexpr int UB = kCodes<T> ? 1 : U;       // halves of 32 tokens that share a softmax step (registers)
   constexpr int C = Tile::kChunks / 256;      // chunks of keys (and of values) a thread unpacks
   constexpr int KG = D == 64 ? 1 : 2;         // groups that a thread's dwords of keys belong to
@@ -1007,7 +1025,7 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
   const int row = wrow + n < rows ? wrow + n : rows - 1;
   const int qi = row / a.grp, head = hk * a.grp + row - qi * a.grp;
   const int pos = past + qi;
-  Frag qf[KS][NP];
+  KFrag qf[KS][NQ];
   float qs[G];
   QueryRow<T, KS, 16> raw_q;
   raw_q.load(static_cast<const T*>(a.q) + (tile.q0 + qi) * a.ldq_t + head * a.ldq_h + 8 * h);
@@ -1068,12 +1086,12 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
           r.vs[x][2 + c] &= keep;
         }
     }
-    Frag* kd = t.k + ((kt >> 5) * KS) * 64 + (kt & 31) + (qq & 1) * 32;
+    KFrag* kd = t.k + ((kt >> 5) * KS) * 64 + (kt & 31) + (qq & 1) * 32;
 #pragma unroll
     for (int c = 0; c < C; ++c) kd[(2 * (k0 + c) + (qq >> 1)) * 64] = O::key(r.k[c], r.ks[c / 2]);
     const uint32_t s[4] = {r.vs[0][0], r.vs[0][1], r.vs[1][0], r.vs[1][1]};
     const uint32_t z[4] = {r.vs[0][2], r.vs[0][3], r.vs[1][2], r.vs[1][3]};
-    Frag* vd = t.v + (2 * vg * (TT / 16) + sub) * 64 + u0 * 32 + n16;
+    VFrag* vd = t.v + (2 * vg * (TT / 16) + sub) * 64 + u0 * 32 + n16;
     if constexpr (D == 64) {  // nibbles 2 (qq >> 1) and the next, moved to the place of 0 and 1
       uint32_t u[4];
 #pragma unroll
@@ -1128,7 +1146,7 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
         x[0] = f32x16{};
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          Frag kf[4];
+          KFrag kf[4];
 #pragma unroll
           for (int k = 0; k < 4; ++k) kf[k] = t.k[(h0 * KS + 4 * g + k) * 64 + lane];
           __builtin_amdgcn_sched_barrier(0);
@@ -1136,7 +1154,7 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int p = NP - 1; p >= 0; --p) sc = O::mma(kf[k], qf[4 * g + k][p], sc);
+            for (int p = NQ - 1; p >= 0; --p) sc = mma(kf[k], qf[4 * g + k][p], sc);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const f32x4 s4 = *reinterpret_cast<const f32x4*>(&t.ks[g][32 * h0 + 8 * q + 4 * h]);
@@ -1145,10 +1163,11 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
             for (int e = 0; e < 4; ++e)
               x[0][4 * q + e] = __builtin_fmaf(s4[e], sc[4 * q + e], __builtin_fmaf(l4[e], qs[g], x[0][4 * q + e]));
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       } else {
         // every operand is on its way before the first product waits for one
-        Frag kf[UB][KS];
+        KFrag kf[UB][KS];
 #pragma unroll
         for (int u = 0; u < UB; ++u)
 #pragma unroll
@@ -1158,16 +1177,17 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
         for (int u = 0; u < UB; ++u) {
           x[u] = f32x16{};
 #pragma unroll
-          for (int k = 0; k < KS; ++k) x[u] = O::mma(kf[u][k], qf[k][0], x[u]);
+          for (int k = 0; k < KS; ++k) x[u] = mma(kf[u][k], qf[k][0], x[u]);
         }
       }
-      Frag vf[2][DT];
-      auto load_values_of = [&](int i, Frag (&f)[DT]) {  // tokens 16 i .. of the half (or halves)
+      constexpr int VB = kCodes<T> ? 1 : 2;  // sets of operands that registers have room for
+      VFrag vf[VB][DT];
+      auto load_values_of = [&](int i, VFrag (&f)[DT]) {  // tokens 16 i .. of the half (or halves)
 #pragma unroll
         for (int d = 0; d < DT; ++d) f[d] = t.v[(d * (TT / 16) + 2 * h0 + i) * 64 + lane];
       };
       __builtin_amdgcn_sched_barrier(0);
-      load_values_of(0, vf[0]);
+      if constexpr (!kCodes<T>) load_values_of(0, vf[0]);
       __builtin_amdgcn_sched_barrier(0);
       if (edge) {  // the row sees tokens from + 4 h + t0 .. upto + 4 h + t0
         const int last = pos < hi - 1 ? pos : hi - 1, upto = last - t0 - 4 * h - 32 * h0;
@@ -1200,7 +1220,8 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
       const float base = m == -__builtin_inff() ? 0.f : m;
 #pragma unroll
       for (int i = 0; i < 2 * UB; ++i) {
-        if (i + 1 < 2 * UB) load_values_of(i + 1, vf[(i + 1) & 1]);
+        if (VB == 2 && i + 1 < 2 * UB) load_values_of(i + 1, vf[(i + 1) % VB]);
+        if (kCodes<T>) load_values_of(i, vf[0]);
         const int u = i >> 1, s = i & 1;
         float p[8];
 #pragma unroll
@@ -1208,7 +1229,7 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
           p[e] = weight_of<T>(x[u][8 * s + e], rs, base);
           if constexpr (kCodes<T>) l += p[e];
         }
-        Frag pf[NP];
+        VFrag pf[NP];
         if constexpr (!kCodes<T>) {
           parts_of(p, pf);
           l = add_weights(p, pf, l);
@@ -1233,7 +1254,7 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
 #pragma unroll
           for (int d = 2 * g; d < 2 * g + 2; ++d)
 #pragma unroll
-            for (int q = NP - 1; q >= 0; --q) o[d] = O::mma(vf[i & 1][d], pf[q], o[d]);
+            for (int q = NP - 1; q >= 0; --q) o[d] = mma(vf[i % VB][d], pf[q], o[d]);
         }
       }
     }
@@ -1313,9 +1334,12 @@ __global__ __launch_bounds__(256, D == 256 || (kCodes<T> && D == 128) ? 1 : 2) v
         for (int e = 0; e < 4; ++e) o[i / 4][4 * (i % 4) + e] = __builtin_fmaf(v[i][e], f, o[i / 4][4 * (i % 4) + e]);
     }
   }
-  if (!busy || wrow + n >= rows) return;
+  int mine = wrow + n;
+  asm volatile("" : "+v"(mine));  // its place is computed again, not held through the loop
+  if (!busy || mine >= rows) return;
+  const int token = (int)((unsigned)mine / (unsigned)a.grp);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  T* out = static_cast<T*>(a.out) + ((tile.q0 + qi) * ((int64_t)a.Hkv * a.grp) + head) * D;
+  T* out = static_cast<T*>(a.out) + ((tile.q0 + token) * ((int64_t)a.Hkv * a.grp) + hk * a.grp + mine - token * a.grp) * D;
 #pragma unroll
   for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -1353,16 +1377,15 @@ void plan_grid(int64_t T, int64_t B, int Hkv, int grp, int R, int64_t rows, int6
   grid = tiles + (fill ? fill + Hkv : 0);
 }
 
-Plan plan_of(bool codes, int D, int64_t T, int64_t B, int Hkv, int grp, int64_t max_query, int64_t max_context, int64_t window) {
+Plan plan_of(int kind, int D, int64_t T, int64_t B, int Hkv, int grp, int64_t max_query, int64_t max_context, int64_t window) {
   Plan p{};
   const int64_t rows = (max_query < T ? max_query : T) * grp;  // of a request
   int64_t span = max_context;
   if (window > 0 && span > window + 128) span = window + 128;
-  const bool wide = codes && D == 256;  // three parts of 32 such queries pass the registers
-  p.rt = rows > 16 && !wide ? 2 : 1;
-  p.rows = rows > kFewRows && !wide;
-  p.ahead = few_ahead(codes, D, p.rt, B * Hkv * cdiv(span, 32) <= 8192);  // 256 blocks of 8 waves, four steps each
-  const int most = few_fill(codes, D, p.rt, p.ahead);
+  p.rt = rows > 16 && few_pairs(kind, D) ? 2 : 1;
+  p.rows = rows > kFewRows && !(kind == 2 && D == 256);  // three parts of 32 such queries pass the registers
+  p.ahead = few_ahead(kind, D, p.rt, B * Hkv * cdiv(span, 32) <= 8192);  // 256 blocks of 8 waves, four steps each
+  const int most = few_fill(kind, D, p.rt, p.ahead);
   if (p.rows && B <= 1) p.rt = 0;
   if (p.rt)
     plan_grid(T, B, Hkv, grp, 16 * p.rt, rows < kFewRows ? rows : kFewRows, cdiv(span, 32) + 1, kFewWhole, kFewLeast, most,
@@ -1382,7 +1405,7 @@ size_t space_of(const Plan& p, int D) {  // the kernels' parts, which run one af
 
 template <class T, int D>
 int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
-  constexpr bool wide = kCodes<T> && D == 256;
+  constexpr bool wide = kKind<T> == 2 && D == 256;
   if constexpr (!wide)
     if (p.rows) {
       a.part_ml = reinterpret_cast<float2*>(a.part_o + p.grid_rows * 128 * D);
@@ -1408,9 +1431,9 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
     auto go = [&](auto rt, auto ahead) {
       constexpr int RT = decltype(rt)::value;
       constexpr bool AHEAD = decltype(ahead)::value;
-      if constexpr (few_ahead(kCodes<T>, D, RT, AHEAD) == AHEAD)  // the forms that a plan takes
+      if constexpr (few_ahead(kKind<T>, D, RT, AHEAD) == AHEAD)  // the forms that a plan takes
         hipLaunchKernelGGL((k_attend_few<T, D, RT, AHEAD>), dim3((unsigned)p.grid_few),
-                           dim3(64 * few_block(kCodes<T>, D, RT, AHEAD)), 0, s, a.starts, a.context, a.T, a.B, a.Hkv, a.grp,
+                           dim3(64 * few_block(kKind<T>, D, RT, AHEAD)), 0, s, a.starts, a.context, a.T, a.B, a.Hkv, a.grp,
                            a.reach, a.window, a.blocks, a);
     };
     auto go_rows = [&](auto rt) {
@@ -1419,13 +1442,13 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
       else
         go(rt, std::false_type{});
     };
-    if constexpr (wide) {
-      go_rows(std::integral_constant<int, 1>{});
-    } else {
+    if constexpr (few_pairs(kKind<T>, D)) {
       if (p.rt == 1)
         go_rows(std::integral_constant<int, 1>{});
       else
         go_rows(std::integral_constant<int, 2>{});
+    } else {
+      go_rows(std::integral_constant<int, 1>{});
     }
   }
   return hip_check(hipGetLastError(), "k_attend launch");
@@ -1455,9 +1478,12 @@ using namespace qs;
 extern "C" size_t qs_kv4_attend_workspace_bytes(int64_t T, int64_t B, int Hkv, int Hq, int D, int64_t page_size,
                                                 int64_t max_query, int64_t max_context, int64_t window) {
   if (check_sizes(T, B, Hkv, Hq, D, page_size) != QS_OK) return 0;
-  const size_t f16 = space_of(plan_of(false, D, T, B, Hkv, Hq / Hkv, max_query, max_context, window), D);
-  const size_t f32 = space_of(plan_of(true, D, T, B, Hkv, Hq / Hkv, max_query, max_context, window), D);
-  return f16 > f32 ? f16 : f32;
+  size_t most = 0;
+  for (int kind = 0; kind < 3; ++kind) {
+    const size_t bytes = space_of(plan_of(kind, D, T, B, Hkv, Hq / Hkv, max_query, max_context, window), D);
+    most = bytes > most ? bytes : most;
+  }
+  return most;
 }
 
 extern "C" int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ldq_h, const uint8_t* cache,
@@ -1478,7 +1504,7 @@ extern "C" int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ld
   if (ldq_t % per16 || ldq_h % per16 || !aligned(q, 16) || !aligned(out, 16) || !aligned(cache, 16))
     return fail(QS_ERR_INVALID, "kv4_attend: 16-byte alignment");
   const int grp = Hq / Hkv;
-  const Plan p = plan_of(dtype == QS_F32, D, T, B, Hkv, grp, max_query, max_context, window);
+  const Plan p = plan_of(dtype == QS_F32 ? 2 : dtype == QS_F16 ? 1 : 0, D, T, B, Hkv, grp, max_query, max_context, window);
   const size_t need = space_of(p, D);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QS_ERR_INVALID, "kv4_attend: workspace of qs_kv4_attend_workspace_bytes() bytes, 16-byte aligned");
