@@ -522,36 +522,42 @@ __device__ __forceinline__ bool last_part(const AttendArgs& a, const Work& w, in
 }
 
 // ---- few rows --------------------------------------------------------------------------------
-// ahead: registers hold the next step's codes too, which hides a load's time where few waves run; the
-// other form leaves room for twice the waves where their number does that, in blocks of half the
-// size, which share out ragged requests more evenly.
+// Forms of the kernel.  kAhead: registers hold the next step's codes too, which hides a load's time
+// where few waves run.  kLean: room for up to twice the waves where their number does that, in blocks
+// of half the size, which share out ragged requests more evenly.  kDeep: the same in blocks of eight
+// waves, which leave half the parts to join where long contexts of few requests are cut into dozens.
+enum { kAhead, kLean, kDeep };
 constexpr bool few_wide(int kind, int D, int rt) { return D * rt >= (kind == 2 ? 256 : 512); }
-constexpr int few_waves(int kind, int D, int rt, bool ahead) {  // a SIMD, as the registers allow
+constexpr int few_waves(int kind, int D, int rt, int form) {  // a SIMD, as the registers allow
   if (few_wide(kind, D, rt)) return 1;
-  return ahead ? 2 : D * rt <= 64 || (kind == 0 && D * rt <= 128) ? 4 : kind == 1 && D * rt <= 128 ? 3 : 2;
+  return form == kAhead ? 2 : D * rt <= 64 || (kind == 0 && D * rt <= 128) ? 4 : kind == 1 && D * rt <= 128 ? 3 : 2;
 }
-constexpr int few_block(int kind, int D, int rt, bool ahead) {  // waves of a block
-  return few_wide(kind, D, rt) || !ahead ? 4 : 8;
+constexpr int few_block(int form) { return form == kLean ? 4 : 8; }  // waves of a block
+constexpr int few_fill(int kind, int D, int rt, int form) {          // blocks that run at once
+  return 1024 * few_waves(kind, D, rt, form) / few_block(form);
 }
-constexpr int few_fill(int kind, int D, int rt, bool ahead) {  // blocks that run at once
-  return 1024 * few_waves(kind, D, rt, ahead) / few_block(kind, D, rt, ahead);
+constexpr int few_form(int kind, int D, int rt, bool few_steps, bool few_tiles) {
+  if (few_wide(kind, D, rt) || D == 256 || (kind == 1 && D * rt == 256)) return kLean;
+  const int waves = few_waves(kind, D, rt, kLean);
+  if (few_steps || waves == 2) return kAhead;
+  return !few_tiles ? kLean : waves == 4 ? kDeep : kAhead;
 }
-// Where both forms exist, `few steps` takes the first.
-constexpr bool few_ahead(int kind, int D, int rt, bool few_steps) {
-  if (few_wide(kind, D, rt) || D == 256 || (kind == 1 && D * rt == 256)) return false;
-  return few_steps || few_waves(kind, D, rt, false) == few_waves(kind, D, rt, true);
+constexpr bool few_used(int kind, int D, int rt, int form) {
+  return form == few_form(kind, D, rt, true, true) || form == few_form(kind, D, rt, false, true) ||
+         form == few_form(kind, D, rt, false, false);
 }
 // Whether registers hold two tiles of 16 rows.
 constexpr bool few_pairs(int kind, int D) { return kind == 0 || D < 256; }
 constexpr int kFewLeast = 16, kFewWhole = 32;    // steps of a part at least, steps that stay whole
 constexpr int kRowsLeast = 4, kRowsWhole = 8, kRowsFill = 512;
 
-template <class T, int D, int RT, bool AHEAD>
-__global__ __launch_bounds__((64 * few_block(kKind<T>, D, RT, AHEAD)), (few_waves(kKind<T>, D, RT, AHEAD))) void k_attend_few(
+template <class T, int D, int RT, int FORM>
+__global__ __launch_bounds__(64 * few_block(FORM), (few_waves(kKind<T>, D, RT, FORM))) void k_attend_few(
     const int* starts, const int* context, int tokens, int requests, int Hkv, int grp, int reach, int window, int blocks, AttendArgs a) {
   a.starts = starts, a.context = context, a.T = tokens, a.B = requests, a.Hkv = Hkv, a.grp = grp, a.reach = reach;
   a.window = window, a.blocks = blocks;
-  constexpr int NW = few_block(kKind<T>, D, RT, AHEAD);
+  constexpr int NW = few_block(FORM);
+  constexpr bool AHEAD = FORM == kAhead;
   using O = Ops<T>;
   typedef typename O::KFrag KFrag;
   typedef typename O::VFrag VFrag;
@@ -1360,7 +1366,7 @@ constexpr int kSyncWords = 8192;  // of the workspace's start, one a block
 struct Plan {
   int rt;           // 16-row tiles of k_attend_few, 0: not used
   bool rows;        // k_attend_rows runs
-  bool ahead;       // which form of k_attend_few
+  int form;         // of k_attend_few
   int64_t grid_few, grid_rows;
   int fill_few, fill_rows;  // blocks that parts fill, 0: no parts
 };
@@ -1384,9 +1390,11 @@ Plan plan_of(int kind, int D, int64_t T, int64_t B, int Hkv, int grp, int64_t ma
   if (window > 0 && span > window + 128) span = window + 128;
   p.rt = rows > 16 && few_pairs(kind, D) ? 2 : 1;
   p.rows = rows > kFewRows && !(kind == 2 && D == 256);  // three parts of 32 such queries pass the registers
-  p.ahead = few_ahead(kind, D, p.rt, B * Hkv * cdiv(span, 32) <= 8192);  // 256 blocks of 8 waves, four steps each
-  const int most = few_fill(kind, D, p.rt, p.ahead);
-  if (p.rows && B <= 1) p.rt = 0;
+  // few steps: 256 blocks of 8 waves, four each; few tiles: each cut into eight parts or more
+  p.form = few_form(kind, D, p.rt, B * Hkv * cdiv(span, 32) <= 8192, B * Hkv <= 64);
+  const int most = few_fill(kind, D, p.rt, p.form);
+  // the tiles of a few requests' few rows find room beside the others; a launch of their own costs more
+  if (p.rows && B * Hkv <= 128) p.rt = 0;
   if (p.rt)
     plan_grid(T, B, Hkv, grp, 16 * p.rt, rows < kFewRows ? rows : kFewRows, cdiv(span, 32) + 1, kFewWhole, kFewLeast, most,
               p.grid_few, p.fill_few);
@@ -1428,19 +1436,19 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
     a.blocks = p.fill_few;
     a.least = kFewLeast;
     a.whole = kFewWhole;
-    auto go = [&](auto rt, auto ahead) {
-      constexpr int RT = decltype(rt)::value;
-      constexpr bool AHEAD = decltype(ahead)::value;
-      if constexpr (few_ahead(kKind<T>, D, RT, AHEAD) == AHEAD)  // the forms that a plan takes
-        hipLaunchKernelGGL((k_attend_few<T, D, RT, AHEAD>), dim3((unsigned)p.grid_few),
-                           dim3(64 * few_block(kKind<T>, D, RT, AHEAD)), 0, s, a.starts, a.context, a.T, a.B, a.Hkv, a.grp,
-                           a.reach, a.window, a.blocks, a);
+    auto go = [&](auto rt, auto form) {
+      constexpr int RT = decltype(rt)::value, FORM = decltype(form)::value;
+      if constexpr (few_used(kKind<T>, D, RT, FORM))
+        hipLaunchKernelGGL((k_attend_few<T, D, RT, FORM>), dim3((unsigned)p.grid_few), dim3(64 * few_block(FORM)), 0, s, a.starts,
+                           a.context, a.T, a.B, a.Hkv, a.grp, a.reach, a.window, a.blocks, a);
     };
     auto go_rows = [&](auto rt) {
-      if (p.ahead)
-        go(rt, std::true_type{});
+      if (p.form == kAhead)
+        go(rt, std::integral_constant<int, kAhead>{});
+      else if (p.form == kLean)
+        go(rt, std::integral_constant<int, kLean>{});
       else
-        go(rt, std::false_type{});
+        go(rt, std::integral_constant<int, kDeep>{});
     };
     if constexpr (few_pairs(kKind<T>, D)) {
       if (p.rt == 1)
