@@ -536,15 +536,14 @@ constexpr int few_block(int form) { return form == kLean ? 4 : 8; }  // waves of
 constexpr int few_fill(int kind, int D, int rt, int form) {          // blocks that run at once
   return 1024 * few_waves(kind, D, rt, form) / few_block(form);
 }
-constexpr int few_form(int kind, int D, int rt, bool few_steps, bool few_tiles) {
-  if (few_wide(kind, D, rt) || D == 256 || (kind == 1 && D * rt == 256)) return kLean;
+constexpr int few_form(int kind, int D, int rt, bool few_steps, bool few_tiles, bool short_tiles) {
+  if (short_tiles || few_wide(kind, D, rt) || D == 256 || (kind == 1 && D * rt == 256)) return kLean;
   const int waves = few_waves(kind, D, rt, kLean);
   if (few_steps || waves == 2) return kAhead;
   return !few_tiles ? kLean : waves == 4 ? kDeep : kAhead;
 }
 constexpr bool few_used(int kind, int D, int rt, int form) {
-  return form == few_form(kind, D, rt, true, true) || form == few_form(kind, D, rt, false, true) ||
-         form == few_form(kind, D, rt, false, false);
+  return form == kLean || form == few_form(kind, D, rt, true, true, false) || form == few_form(kind, D, rt, false, true, false);
 }
 // Whether registers hold two tiles of 16 rows.
 constexpr bool few_pairs(int kind, int D) { return kind == 0 || D < 256; }
@@ -1390,8 +1389,10 @@ Plan plan_of(int kind, int D, int64_t T, int64_t B, int Hkv, int grp, int64_t ma
   if (window > 0 && span > window + 128) span = window + 128;
   p.rt = rows > 16 && few_pairs(kind, D) ? 2 : 1;
   p.rows = rows > kFewRows && !(kind == 2 && D == 256);  // three parts of 32 such queries pass the registers
-  // few steps: 256 blocks of 8 waves, four each; few tiles: each cut into eight parts or more
-  p.form = few_form(kind, D, p.rt, B * Hkv * cdiv(span, 32) <= 8192, B * Hkv <= 64);
+  // few steps: 256 blocks of 8 waves, four each; few tiles: each cut into eight parts or more; short
+  // ones: more than run at once in blocks of eight waves, of which each would have a step at most
+  const int64_t steps = cdiv(span, 32), tiles = (T * grp / (16 * p.rt) + B + 1) * Hkv;
+  p.form = few_form(kind, D, p.rt, B * Hkv * steps <= 8192, B * Hkv <= 64, tiles > 256 && steps <= 8);
   const int most = few_fill(kind, D, p.rt, p.form);
   // the tiles of a few requests' few rows find room beside the others; a launch of their own costs more
   if (p.rows && B * Hkv <= 128) p.rt = 0;
