@@ -6,7 +6,8 @@ call into ``libqstore_hip.so``; there is no CPU fallback.  Submodules:
 
 * ``_native``      -- ctypes binding of ``libqstore_hip.so`` (signatures equal to
   ``include/qstore_hip.h``); raises when the library is missing.
-* ``build``        -- compiles ``csrc/`` for gfx950 into ``libqstore_hip.so``.
+* ``build``        -- compiles ``csrc/`` for gfx950 into ``libqstore_hip.so``, and the torch binding
+  of the short calls (``_qs_torch.so``).
 * ``qrow``         -- int8 row-scaled linears: dequant, W8A16 / fp32 GEMV, batched decode,
   paired SwiGLU, multi-linear launches, fused head + top-2 and its fp32 rerank.
 * ``store``        -- the QStore v3 on-disk format: reader, writer, layout validation.
@@ -23,11 +24,14 @@ call into ``libqstore_hip.so``; there is no CPU fallback.  Submodules:
 * ``expert_queue`` -- expert-major packet queues and their committed scatter.
 * ``expert_cache`` -- paged int8 experts: page store, pinned host tier, HBM slot cache
   (eviction policies, transient prefill, page trace).
+* ``paging``       -- block tables, slot maps and positions of a step from request lengths.
+* ``rotary``       -- rotary positions: both pair layouts, part of a head, scaled contexts.
+* ``kv4``          -- the paged 4-bit KV cache: append, read, and attention over it.
 * ``ops``          -- ``torch.library`` custom ops (``torch.ops.qstore_hip.*``) with fake
   kernels.
 """
 
 from __future__ import annotations
 
-__all__ = ["codecs", "dense_store", "expert_cache", "expert_queue", "lowbit", "moe", "ops", "paged",
-           "provenance", "qrow", "store", "w8a8"]
+__all__ = ["codecs", "dense_store", "expert_cache", "expert_queue", "kv4", "lowbit", "moe", "ops", "paged",
+           "paging", "provenance", "qrow", "rotary", "store", "w8a8"]

@@ -9,7 +9,17 @@
 //
 // o = sum_t p_t v_t / sum_t p_t with p_t = 2^(x_t - m), x the scores in units of log2 and m their
 // running maximum, one pass over the cache.  Blocks share the requests' tokens out among themselves
-// (pick_work); where several take parts of one tile's tokens, the last of them to finish joins them.
+// (pick_part); where several take parts of one tile's tokens, the last of them to finish joins them.
+//
+// Measured on an MI355X whose copy reaches 5.1 TB/s and whose 8192^3 bf16 product 1155 TFLOP/s (in
+// brackets with 1231), heads of 128, a call from Python:
+//   1 token over 513, 12 + 2 heads           7.3 us  latency: plan, pages, first codes, 3 steps, join
+//   29 requests up to 8100, 32 + 8 heads    31.5 us  3.5 TB/s; the vector unit unpacks 60% of it
+//   2 contexts of 131000, fp16              68.7 us  4.4 TB/s (65)
+//   11 requests of 5 tokens up to 6001      18.4 us  latency
+//   4095 tokens, 32 + 8 heads                188 us  731 TFLOP/s (171, 801): vector operations 49% and
+//                                                    products 38% of the cycles, hardly at once
+//   chunks of 701, window 1024, fp32 of 64  36.1 us  153 TFLOP/s, the fp32 product's own rate
 #include <type_traits>
 
 #include "qs_kv4.h"
@@ -522,6 +532,8 @@ __device__ __forceinline__ bool last_part(const AttendArgs& a, const Work& w, in
 }
 
 // ---- few rows --------------------------------------------------------------------------------
+// Bound by the codes' bytes and by their unpacking: 176 operations of about 250 for 32 tokens of a head
+// of 128, whatever the number of rows.
 // Forms of the kernel.  kAhead: registers hold the next step's codes too, which hides a load's time
 // where few waves run.  kLean: room for up to twice the waves where their number does that, in blocks
 // of half the size, which share out ragged requests more evenly.  kDeep: the same in blocks of eight
@@ -978,6 +990,9 @@ __global__ __launch_bounds__(64 * few_block(FORM), (few_waves(kKind<T>, D, RT, F
 }
 
 // ---- many rows -------------------------------------------------------------------------------
+// Unpacking once a block of 128 rows costs a wave a quarter of what it costs alone; 32 rows a wave and
+// two waves a SIMD, since a wave alone issues a vector operation only every 7 cycles (64 rows a wave,
+// one a SIMD: 197 us on the prompt of 4095 where this takes 171).
 // 64 tokens (32 of heads of 256) unpacked in LDS, each eight values along a product's sum in 16
 // bytes, in the order in which v_mfma_f32_32x32x16 takes them:
 //   keys   [token / 32][d / 16][d / 8 & 1][token & 31]

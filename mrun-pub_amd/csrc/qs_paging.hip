@@ -11,7 +11,8 @@
 //                     the step can be planned again, and captured into a graph.
 //   k_release_pages : finished requests' pages back to the ring's end, in request order.
 //
-// Bound by the launch for a few requests, by 20 bytes of output a token for many.
+// Bound by latency: 7 requests take 3.9 us, 511 requests with 48,000 tokens 5.5 (two chunks of 256
+// requests and four tokens a thread took 8.7).
 #include "qs_common.h"
 
 namespace qs {

@@ -6,7 +6,8 @@
 //
 // y1 = x1 c - x2 s, y2 = x2 c + x1 s, products and sums each rounded in fp32 and the result once to
 // x's type; the inverse (which is also the gradient) turns by -s.  Bound by memory: every value is
-// read once and written once, and a block's threads share their tokens' angles through LDS.
+// read once and written once, and a block's threads share their tokens' angles through LDS.  8191
+// tokens of 40 heads of 128 (168 MB) take 35.6 us, 4.7 TB/s of a copy's 5.1; one token 2.4.
 #include "qs_rotary.h"
 #include "qs_values.h"
 
