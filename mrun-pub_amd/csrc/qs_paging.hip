@@ -6,7 +6,7 @@
 // the ranks.
 //
 //   k_plan_step     : one launch.  Every block redoes the sums over all requests (8 bytes each, in
-//                     LDS for up to kPlanRequests at a time) and then fills its own tokens, so no
+//                     LDS for kPlanThreads at a time) and then fills its own tokens, so no
 //                     block waits for another.  The ring's new state goes to a place of its own:
 //                     the step can be planned again, and captured into a graph.
 //   k_release_pages : finished requests' pages back to the ring's end, in request order.
