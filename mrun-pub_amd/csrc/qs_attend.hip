@@ -12,7 +12,7 @@
 // (pick_part); where several take parts of one tile's tokens, the last of them to finish joins them.
 //
 // Measured on an MI355X whose copy reaches 5.1 TB/s and whose 8192^3 bf16 product 1155 TFLOP/s (in
-// brackets with 1231), heads of 128, a call from Python:
+// brackets other cards, not rated), heads of 128, a call from Python:
 //   1 token over 513, 12 + 2 heads           7.3 us  latency: plan, pages, first codes, 3 steps, join
 //   29 requests up to 8100, 32 + 8 heads    31.5 us  3.5 TB/s; the vector unit unpacks 60% of it
 //   2 contexts of 131000, fp16              68.7 us  4.4 TB/s (65)
