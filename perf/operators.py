@@ -299,7 +299,7 @@ def _quantize(x):
     t, h, d = x.shape
     g = x.float().view(t, h, d // GROUP, GROUP)
     low, high = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-    lo, sc = low.half(), ((high - low) / torch.full_like(low, 15.0)).half()  # a scalar would be a product with 1/15
+    lo, sc = low.half(), ((high - low) / 15.0).half()
     q = torch.where(sc > 0, torch.round((g - lo.float()) / sc.float()).clamp_(0, 15), 0.0).to(torch.uint8).view(t, h, d)
     return q[..., 0::2] | (q[..., 1::2] << 4), sc.squeeze(-1), lo.squeeze(-1)
 
