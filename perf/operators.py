@@ -284,6 +284,9 @@ def prepare(case: dict, seed: int) -> dict:
             from mrun_pub_amd import kv4
 
             s["cache"] = kv4.KV4Cache(layers=1, kv_heads=hkv, head_dim=d, pages=pages, page_size=P, device=DEV)
+            # what the plain codes stand for is coded as these codes again: both sides attend over one cache,
+            # whatever the rounding of the scales
+            k, v = (_values(*_quantize(x)) for x in (k, v))
             kv4.append(s["cache"], 0, k, v, torch.arange(pages * P, device=DEV))
         else:
             s["kc"], s["ks"], s["kl"] = _quantize(k)
