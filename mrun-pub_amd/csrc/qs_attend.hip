@@ -23,6 +23,7 @@
 #include <type_traits>
 
 #include "qs_kv4.h"
+#include "qs_span.h"
 #include "qs_values.h"
 
 namespace qs {
@@ -429,19 +430,6 @@ __device__ __forceinline__ Work pick_work(const AttendArgs& a, float* s_sum, Wor
   return t;
 }
 
-// Tokens [lo, hi) that some of the rows see, which stand at pos_min .. pos_max.
-struct Span {
-  int lo, hi;
-};
-__device__ __forceinline__ Span span_of(const AttendArgs& a, int b, int pos_min, int pos_max) {
-  Span s;
-  s.hi = pos_max + 1;
-  if (s.hi > a.reach) s.hi = a.reach;
-  s.lo = a.window > 0 && pos_min - a.window + 1 > 0 ? pos_min - a.window + 1 : 0;
-  if (b >= a.B || s.hi < s.lo) s.hi = s.lo;
-  return s;
-}
-
 // The lane's query row: KS pieces of 8 values, STRIDE apart, as operands.
 template <class T, int KS, int STRIDE>
 struct QueryRow {
@@ -587,7 +575,7 @@ __global__ __launch_bounds__(64 * few_block(FORM), (few_waves(kKind<T>, D, RT, F
   const int past = tile.ctx - tile.n;  // position of the first new token
   const int r_last = tile.row0 + R - 1 < rows ? tile.row0 + R - 1 : rows - 1;
   const int pos_min = past + tile.row0 / a.grp, pos_max = past + r_last / a.grp;
-  const Span span = span_of(a, tile.b, pos_min, pos_max);
+  const Span span = span_of(pos_min, pos_max, a.window, a.reach, tile.b < a.B);
   const int lo = span.lo, hi = span.hi;
 
   // this block's steps of 32 tokens, of which the wave takes every NW-th
@@ -1034,7 +1022,7 @@ __global__ __launch_bounds__(256, D == 256 || (kKind<T> == 2 && D == 128) ? 1 : 
   const int hk = tile.hk, rows = tile.n * a.grp;
   const int past = tile.ctx - tile.n;
   const int r_last = tile.row0 + R - 1 < rows ? tile.row0 + R - 1 : rows - 1;
-  const Span span = span_of(a, tile.b, past + tile.row0 / a.grp, past + r_last / a.grp);
+  const Span span = span_of(past + tile.row0 / a.grp, past + r_last / a.grp, a.window, a.reach, tile.b < a.B);
   const int lo = span.lo, hi = span.hi;
 
   // the wave's 32 rows, and the positions between which they stand
