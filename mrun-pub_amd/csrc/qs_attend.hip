@@ -65,13 +65,18 @@ struct AttendArgs {
 // both 16-bit types hold exactly: q.k = s (q.code) + lo sum(q) a group, and for the output the
 // weights are p s, with p lo summed beside.  fp16 queries are operands as they are, fp32 ones sums of
 // three bf16 numbers (8 bits each, all of fp32's 24); p s is a sum of two or three bf16 numbers.
-// Three instructions of the 16-bit rate replace the fp32 instruction's sixteenfold time.
+// Three instructions of the 16-bit rate replace the fp32 instruction's sixteenfold time.  Codes are
+// 0..15 and lo is near -7.5 s, so the two sums of an output are large and cancel: fp32 adds p lo to the
+// products' sum at every step, where both are still small, which leaves the result as exact as values
+// multiplied in fp32 (a prompt of 300, heads of 128: 3.4e-7 off 64 bits, 8.5e-7 with two sums to the end).
 constexpr uint32_t kNibbles = 0x0f0f0f0fu;
 
 template <class T>
 constexpr int kKind = __is_same(T, __bf16) ? 0 : sizeof(T) == 2 ? 1 : 2;
 template <class T>
 constexpr bool kCodes = kKind<T> != 0;
+template <class T>
+constexpr bool kFold = kKind<T> == 2;  // p lo joins the products' sum at every step
 template <class T>
 constexpr int kQueryParts = kKind<T> == 2 ? 3 : 1;
 template <class T>
@@ -659,7 +664,7 @@ __global__ __launch_bounds__(64 * few_block(FORM), (few_waves(kKind<T>, D, RT, F
   }
 
   f32x4 o[RT][G][4];
-  float m[RT], l[RT], ol[RT][G];  // ol: codes' sum of p lo
+  float m[RT], l[RT], ol[RT][G];  // ol: the codes' sum of p lo, if it has one of its own
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m[rt] = -__builtin_inff();
@@ -769,7 +774,7 @@ __global__ __launch_bounds__(64 * few_block(FORM), (few_waves(kKind<T>, D, RT, F
         l[rt] *= f;
 #pragma unroll
         for (int g = 0; g < G; ++g) {
-          if constexpr (kCodes<T>) ol[rt][g] *= f;
+          if constexpr (kCodes<T> && !kFold<T>) ol[rt][g] *= f;
 #pragma unroll
           for (int j = 0; j < 4; ++j) o[rt][g][j] *= f;
         }
@@ -803,14 +808,21 @@ __global__ __launch_bounds__(64 * few_block(FORM), (few_waves(kKind<T>, D, RT, F
       if constexpr (kCodes<T>) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          float w[8];
+          float w[8], low = kFold<T> ? 0.f : ol[rt][g];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int up = 16 * (e & 1);
             w[e] = p[rt][e] * f16_bits_to_f32((uint16_t)(s[e >> 1] >> up));
-            ol[rt][g] = __builtin_fmaf(p[rt][e], f16_bits_to_f32((uint16_t)(z[e >> 1] >> up)), ol[rt][g]);
+            low = __builtin_fmaf(p[rt][e], f16_bits_to_f32((uint16_t)(z[e >> 1] >> up)), low);
           }
           parts_of(w, pf[rt]);
+          if constexpr (kFold<T>) {
+            low = quad_sum(low);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[rt][g][j] += low;
+          } else {
+            ol[rt][g] = low;
+          }
         }
       }
       auto product = [&](const VFrag& vf, int j) {
@@ -868,12 +880,12 @@ __global__ __launch_bounds__(64 * few_block(FORM), (few_waves(kKind<T>, D, RT, F
     if (qq == 0) s_ml[wave][n] = {m[rt], sum};
 #pragma unroll
     for (int g = 0; g < G; ++g) {
-      const float add = kCodes<T> ? quad_sum(ol[rt][g]) : 0.f;
+      const float add = kCodes<T> && !kFold<T> ? quad_sum(ol[rt][g]) : 0.f;
       if (rt * 16 + n >= live) continue;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         f32x4 w = {o[rt][g][0][r], o[rt][g][1][r], o[rt][g][2][r], o[rt][g][3][r]};
-        if constexpr (kCodes<T>) w += add;
+        if constexpr (kCodes<T> && !kFold<T>) w += add;
         *reinterpret_cast<f32x4*>(&s_o[wave][n][64 * g + 16 * qq + 4 * r]) = w;
       }
     }
@@ -1220,12 +1232,16 @@ __global__ __launch_bounds__(256, D == 256 || (kKind<T> == 2 && D == 128) ? 1 : 
         const float f = to == -__builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(m - to);
         l *= f;
 #pragma unroll
-        for (int g = 0; g < G; ++g) ol[g] *= f;
+        for (int g = 0; g < G; ++g)
+          if constexpr (!kFold<T>) ol[g] *= f;
 #pragma unroll
         for (int d = 0; d < DT; ++d) o[d] *= f;
         m = to;
       }
       const float base = m == -__builtin_inff() ? 0.f : m;
+      if constexpr (kFold<T>)
+#pragma unroll
+        for (int g = 0; g < G; ++g) ol[g] = 0.f;
 #pragma unroll
       for (int i = 0; i < 2 * UB; ++i) {
         if (VB == 2 && i + 1 < 2 * UB) load_values_of(i + 1, vf[(i + 1) % VB]);
@@ -1265,6 +1281,15 @@ __global__ __launch_bounds__(256, D == 256 || (kKind<T> == 2 && D == 128) ? 1 : 
             for (int q = NP - 1; q >= 0; --q) o[d] = mma(vf[i % VB][d], pf[q], o[d]);
         }
       }
+      if constexpr (kFold<T>)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const float low = pair_sum(ol[g]);
+#pragma unroll
+          for (int d = 2 * g; d < 2 * g + 2; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] += low;
+        }
     }
   };
 
@@ -1294,7 +1319,7 @@ __global__ __launch_bounds__(256, D == 256 || (kKind<T> == 2 && D == 128) ? 1 : 
 
   // a wave has its rows to itself: parts are stored as the registers lie
   l = pair_sum(l);
-  if constexpr (kCodes<T>)
+  if constexpr (kCodes<T> && !kFold<T>)
 #pragma unroll
     for (int g = 0; g < G; ++g) {
       const float add = pair_sum(ol[g]);

@@ -57,3 +57,27 @@ def test_a_plan_that_outgrew_its_table(dev):
     out = kv4.attend(s.q, s.cache, 0, s.tables, p.query_starts, p.context_lens, window=10)
     check_unseen(s, out, 10)
     assert not out[0].any() and out[1].any()
+
+
+@pytest.mark.parametrize("hq,hkv,d,ctx,new", [(8, 4, 64, 1300, 200), (8, 4, 64, 4000, 70), (4, 2, 128, 2200, 100), (4, 2, 128, 300, 300), (4, 2, 64, 700, 700),
+                                              (8, 2, 64, 5000, 1), (8, 2, 128, 9000, 3), (4, 1, 256, 3000, 9)])
+def test_fp32_attention_is_as_exact_as_the_plain_form(dev, hq, hkv, d, ctx, new):
+    """Against 64 bits, in the 2-norm: twice what the plain form in fp32 is off, and what n / 16 roundings
+    of a sum that runs over n tokens, 16 at a time, add to it: each at most 2^-24 of the sum, of no
+    common sign, so sqrt(n / 16) of them.  Codes and lowest values, whose sums cancel, add nothing."""
+    s = Setup(dev, [ctx], [new], hq, hkv, d, 16, torch.float32, seed=ctx)
+    out = f64(s.attend())
+    q, k, v = f64(s.q), s.keys[0], s.values[0]
+    want, _, _ = oa.attend(q, s.keys, s.values, s.starts, s.ctx, d**-0.5)
+    plain = np.zeros_like(want)
+    for i in range(new):
+        n = ctx - new + i + 1
+        for h in range(hq):
+            kh, vh = (x[:n, h // (hq // hkv)].astype(np.float32) for x in (k, v))
+            x = kh @ q[i, h].astype(np.float32) * np.float32(d**-0.5)
+            w = np.exp(x - x.max())
+            plain[i, h] = (w @ vh) / w.sum()
+    size = np.linalg.norm(want)
+    off, plain_off = np.linalg.norm(out - want) / size, np.linalg.norm(plain - want) / size
+    print(f"off by {off:.2e}, the plain form by {plain_off:.2e}")
+    assert off <= 2 * plain_off + (ctx / 16) ** 0.5 * 2.0**-24
