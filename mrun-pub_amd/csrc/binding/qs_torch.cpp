@@ -107,6 +107,9 @@ at::Tensor part_of(const at::Tensor& whole, at::ScalarType type, int64_t offset,
   return at::Tensor(std::move(impl));
 }
 
+// Values from one entry of a dimension to the next; a dimension of one has no next, whatever its stride.
+int64_t step(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }
+
 at::Tensor vector_of(const at::Tensor& t, at::ScalarType type) {
   if (t.scalar_type() == type && t.is_contiguous()) return t;
   return t.to(type).contiguous();
@@ -129,7 +132,7 @@ at::Tensor slots_of(const at::Tensor& t, int64_t tokens) {
 void check_tables(const at::Tensor& t, int64_t requests) {
   REFUSE(t.dim() != 2 || t.scalar_type() != at::kInt || t.size(0) != requests,
          "block tables must be int32 [requests, columns]");
-  REFUSE(t.numel() && t.stride(1) != 1, "block table rows must be contiguous");
+  REFUSE(t.numel() && t.size(1) > 1 && t.stride(1) != 1, "block table rows must be contiguous");
 }
 
 // [tokens, heads, head_dim] with heads aligned to `values` values, copied if it is not.
@@ -138,7 +141,7 @@ at::Tensor heads_of(const at::Tensor& x, const char* name, int64_t tokens, int64
          std::string(name) + " must have shape [" + std::to_string(tokens) + ", heads, " + std::to_string(head_dim) + "]");
   REFUSE(heads >= 0 && x.size(1) != heads, std::string(name) + " must have " + std::to_string(heads) + " heads");
   const auto off = [&](const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % (t.element_size() * values); };
-  if (x.stride(2) == 1 && x.stride(0) % values == 0 && x.stride(1) % values == 0 && !off(x)) return x;
+  if (x.stride(2) == 1 && step(x, 0) % values == 0 && step(x, 1) % values == 0 && !off(x)) return x;
   at::Tensor y = x.contiguous();
   return off(y) ? y.clone() : y;  // a contiguous view may start off the grid
 }
@@ -261,9 +264,9 @@ PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
     if (T == 0 || H == 0) return give(out);
     const at::Tensor& freq = tensor(v[2], "frequencies");
     d.add(freq);
-    check(entry.rotary(x.data_ptr(), code, x.stride(0), x.stride(1), static_cast<int32_t*>(pos.data_ptr()),
+    check(entry.rotary(x.data_ptr(), code, step(x, 0), step(x, 1), static_cast<int32_t*>(pos.data_ptr()),
                        static_cast<double*>(freq.data_ptr()), (int)dim, PyObject_IsTrue(v[4]), PyObject_IsTrue(v[5]),
-                       number(v[6], "magnitude"), out.data_ptr(), out.stride(0), out.stride(1), T, (int)H, (int)D, d.stream()),
+                       number(v[6], "magnitude"), out.data_ptr(), step(out, 0), step(out, 1), T, (int)H, (int)D, d.stream()),
           "qs_rotary");
     return give(out);
   });
@@ -309,10 +312,10 @@ PyObject* append(PyObject*, PyObject* const* v, Py_ssize_t n) {
     int64_t Hq = 0, ldq_t = 0, ldq_h = 0;
     if (has_q) {
       q = heads_of(q, "queries", T, -1, D, 4);
-      Hq = q.size(1), ldq_t = q.stride(0), ldq_h = q.stride(1);
+      Hq = q.size(1), ldq_t = step(q, 0), ldq_h = step(q, 1);
       out = d.empty({T, Hq, D}, q.scalar_type());
     }
-    check(entry.append(k.data_ptr(), k.stride(0), k.stride(1), val.data_ptr(), val.stride(0), val.stride(1),
+    check(entry.append(k.data_ptr(), step(k, 0), step(k, 1), val.data_ptr(), step(val, 0), step(val, 1),
                        code_of(k.scalar_type()), static_cast<int64_t*>(slots.data_ptr()), base, cache.pages, cache.page_size,
                        (int)cache.kv_heads, (int)D, T, has_q ? q.data_ptr() : nullptr, ldq_t, ldq_h, (int)Hq,
                        has_q ? out.data_ptr() : nullptr, turns ? static_cast<int32_t*>(pos.data_ptr()) : nullptr,
@@ -391,7 +394,7 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
                                                      max_context, window);
     at::Tensor space;
     if (need) space = workspace(d, stream, need);
-    check(entry.attend(q.data_ptr(), code_of(q.scalar_type()), q.stride(0), q.stride(1), base, cache.pages, cache.page_size,
+    check(entry.attend(q.data_ptr(), code_of(q.scalar_type()), step(q, 0), step(q, 1), base, cache.pages, cache.page_size,
                        (int)cache.kv_heads, (int)Hq, (int)D, static_cast<int32_t*>(tables.data_ptr()), tables.stride(0), width,
                        static_cast<int32_t*>(starts.data_ptr()), static_cast<int32_t*>(ctx.data_ptr()), B, T, max_query,
                        max_context, (float)scale, window, out.data_ptr(), need ? space.data_ptr() : nullptr, (size_t)need, stream),

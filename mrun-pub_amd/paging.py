@@ -51,7 +51,7 @@ def _pool(ring: torch.Tensor, state: torch.Tensor) -> None:
 def _tables(block_tables: torch.Tensor, requests: int) -> None:
     if block_tables.ndim != 2 or block_tables.dtype != torch.int32 or int(block_tables.shape[0]) != requests:
         raise ValueError("block tables must be int32 [requests, columns]")
-    if block_tables.numel() and block_tables.stride(1) != 1:
+    if block_tables.numel() and block_tables.shape[1] > 1 and block_tables.stride(1) != 1:
         raise ValueError("block table rows must be contiguous")
 
 

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from mrun_pub_amd import kv4, paging
+from mrun_pub_amd import kv4, paging, rotary
 from oracle import attention as oa
 from test_gpu_attention import Setup, f64, i32
 
@@ -81,3 +81,39 @@ def test_fp32_attention_is_as_exact_as_the_plain_form(dev, hq, hkv, d, ctx, new)
     off, plain_off = np.linalg.norm(out - want) / size, np.linalg.norm(plain - want) / size
     print(f"off by {off:.2e}, the plain form by {plain_off:.2e}")
     assert off <= 2 * plain_off + (ctx / 16) ** 0.5 * 2.0**-24
+
+
+def test_strides_of_dimensions_of_one_do_not_matter(dev):
+    """One token, one head or one column: its stride is never used, whatever it is."""
+    s = Setup(dev, [40], [1], 4, 1, 64, 16, torch.bfloat16)
+    want, pos, spec = s.attend(), i32([39], dev), rotary.RotarySpec(64)
+    turned = rotary.apply_rotary(s.q, pos, spec)
+    flat = torch.zeros(4 * 64 + 8, device=dev, dtype=torch.bfloat16)
+    flat[:256] = s.q.flatten()
+    q = flat.as_strided((1, 4, 64), (4 * 64 + 3, 64, 1))
+    assert torch.equal(s.attend(q), want)
+    into = torch.zeros_like(flat)
+    rotary.apply_rotary(q, pos, spec, out=into.as_strided((1, 4, 64), (259, 64, 1)))
+    assert torch.equal(into[:256], turned.flatten()) and not into[256:].any()
+    k = s.k[:1].as_strided((1, 1, 64), (67, 65, 1))
+    a, b = (kv4.KV4Cache(layers=1, kv_heads=1, head_dim=64, pages=1, page_size=16, device=dev) for _ in range(2))
+    slot = torch.tensor([3], device=dev)
+    out = kv4.append(a, 0, k, k, slot, q=q, positions=pos, rotary=spec)
+    assert torch.equal(out, turned)
+    kv4.append(b, 0, s.k[:1], s.k[:1], slot, positions=pos, rotary=spec)
+    assert torch.equal(a.storage, b.storage)
+
+    s = Setup(dev, [9, 5], [1, 1], 4, 1, 64, 16, torch.bfloat16)
+    narrow(s, 1)
+    want = s.attend()
+    s.tables = torch.stack([s.tables[:, 0], s.tables[:, 0]], 1).contiguous().as_strided((2, 1), (2, 7))
+    assert torch.equal(s.attend(), want)
+    ring, state = paging.free_pages(4, dev)
+    new = i32([1, 1], dev)
+    plans = [paging.plan_step(ring, state, t, i32([0, 0], dev), new, page_size=16, tokens=2)
+             for t in (torch.full((2, 1), -1, dtype=torch.int32, device=dev),
+                       torch.full((2, 2), -1, dtype=torch.int32, device=dev).as_strided((2, 1), (2, 5)))]
+    assert all(torch.equal(x, y) for x, y in zip(*plans))
+    done = torch.ones(2, dtype=torch.bool, device=dev)
+    held = torch.zeros(2, 2, dtype=torch.int32, device=dev).as_strided((2, 1), (2, 5))
+    assert paging.release_pages(ring, plans[0].free_state, held, new, done, page_size=16).tolist() == [2, 6, 0]
