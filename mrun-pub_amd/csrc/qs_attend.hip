@@ -1542,6 +1542,8 @@ extern "C" int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ld
     return fail(QS_ERR_INVALID, "kv4_attend: 16-byte alignment");
   const int grp = Hq / Hkv;
   const Plan p = plan_of(dtype == QS_F32 ? 2 : dtype == QS_F16 ? 1 : 0, D, T, B, Hkv, grp, max_query, max_context, window);
+  if ((p.rt && p.grid_few > most_blocks(64 * few_block(p.form))) || (p.rows && p.grid_rows > most_blocks(256)))
+    return fail(QS_ERR_LIMIT, "kv4_attend: %lld query rows need more threads than the 2^32 of a grid", (long long)(T * Hq));
   const size_t need = space_of(p, D);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
     return fail(QS_ERR_INVALID, "kv4_attend: workspace of qs_kv4_attend_workspace_bytes() bytes, 16-byte aligned");

@@ -30,6 +30,8 @@ inline bool aligned(const void* p, int bytes) {
   return (reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes)) == 0;
 }
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Blocks that one launch takes: a grid has fewer than 2^32 threads, and more are cut off without an error.
+inline int64_t most_blocks(int threads) { return (int64_t)UINT32_MAX / threads; }
 
 // ---------------------------------------------------------------------------------
 // device helpers

@@ -201,6 +201,26 @@ __global__ __launch_bounds__(256) void k_kv4_append(AppendArgs a) {
 }
 
 template <class T>
+int launch_append(const AppendArgs& a, int64_t tokens, hipStream_t s) {
+  const int64_t each = most_blocks(256);
+  for (int64_t t0 = 0; t0 < tokens; t0 += each) {
+    AppendArgs part = a;
+    part.k = static_cast<const T*>(a.k) + t0 * a.ldk_t;
+    part.v = static_cast<const T*>(a.v) + t0 * a.ldv_t;
+    if (a.Hq) {
+      part.q = static_cast<const T*>(a.q) + t0 * a.ldq_t;
+      part.q_out = static_cast<T*>(a.q_out) + t0 * a.Hq * a.D;
+    }
+    part.slots = a.slots + t0;
+    if (a.rot) part.pos = a.pos + t0;
+    hipLaunchKernelGGL(k_kv4_append<T>, dim3((unsigned)(tokens - t0 < each ? tokens - t0 : each)), dim3(256), 0, s, part);
+    const int status = hip_check(hipGetLastError(), "k_kv4_append launch");
+    if (status != QS_OK) return status;
+  }
+  return QS_OK;
+}
+
+template <class T>
 __global__ __launch_bounds__(256) void k_kv4_read(const uint8_t* cache, const int64_t* slots, int64_t slots_all, int P,
                                                   int D, int Hkv, int64_t n, T* k_out, T* v_out) {
   const Kv4Layout L(P, D);
@@ -269,17 +289,11 @@ extern "C" int qs_kv4_append(const void* k, int64_t ldk_t, int64_t ldk_h, const 
   const int per16 = 16 / size;
   a.wide = Hq > 0 && aligned(q, 16) && aligned(q_out, 16) && ldq_t % per16 == 0 && ldq_h % per16 == 0 &&
            (size == 4 ? TurnItem<float>::fits(D, rot, interleaved) : TurnItem<__bf16>::fits(D, rot, interleaved));
-  const dim3 grid((unsigned)T), block(256);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (dtype == QS_F32)
-    hipLaunchKernelGGL(k_kv4_append<float>, grid, block, 0, s, a);
-  else if (dtype == QS_BF16)
-    hipLaunchKernelGGL(k_kv4_append<__bf16>, grid, block, 0, s, a);
-  else if (dtype == QS_F16)
-    hipLaunchKernelGGL(k_kv4_append<_Float16>, grid, block, 0, s, a);
-  else
-    return fail(QS_ERR_INVALID, "kv4_append: dtype must be F32, BF16 or F16");
-  return hip_check(hipGetLastError(), "k_kv4_append launch");
+  if (dtype == QS_F32) return launch_append<float>(a, T, s);
+  if (dtype == QS_BF16) return launch_append<__bf16>(a, T, s);
+  if (dtype == QS_F16) return launch_append<_Float16>(a, T, s);
+  return fail(QS_ERR_INVALID, "kv4_append: dtype must be F32, BF16 or F16");
 }
 
 extern "C" int qs_kv4_read(const uint8_t* cache, int64_t pages, int64_t page_size, int Hkv, int D, const int64_t* slots,

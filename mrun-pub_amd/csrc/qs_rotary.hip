@@ -106,13 +106,23 @@ int launch_rotary(RotaryArgs a, hipStream_t s) {
   // tokens of few items share a block, up to 16, whose angles are at most 16 x 1024 x 8 bytes
   a.tokens = (int)(per_token >= 256 ? 1 : 256 / per_token < 16 ? 256 / per_token : 16);
   if (a.tokens * a.rot > 8192) a.tokens = a.rot > 8192 ? 1 : 8192 / a.rot;
-  const int64_t blocks = cdiv(a.T, a.tokens);
   const size_t lds = (size_t)a.tokens * (a.rot / 2) * sizeof(float2);
-  if (wide)
-    hipLaunchKernelGGL(k_rotary_v<T>, dim3((unsigned)blocks), dim3(256), lds, s, a);
-  else
-    hipLaunchKernelGGL(k_rotary_1<T>, dim3((unsigned)blocks), dim3(256), lds, s, a);
-  return hip_check(hipGetLastError(), "k_rotary launch");
+  const int64_t each = most_blocks(256) * a.tokens, all = a.T;  // tokens of a launch
+  for (int64_t t0 = 0; t0 < all; t0 += each) {
+    RotaryArgs part = a;
+    part.x = static_cast<const T*>(a.x) + t0 * a.ldx_t;
+    part.y = static_cast<T*>(a.y) + t0 * a.ldy_t;
+    part.pos = a.pos + t0;
+    part.T = all - t0 < each ? all - t0 : each;
+    const dim3 grid((unsigned)cdiv(part.T, a.tokens));
+    if (wide)
+      hipLaunchKernelGGL(k_rotary_v<T>, grid, dim3(256), lds, s, part);
+    else
+      hipLaunchKernelGGL(k_rotary_1<T>, grid, dim3(256), lds, s, part);
+    const int status = hip_check(hipGetLastError(), "k_rotary launch");
+    if (status != QS_OK) return status;
+  }
+  return QS_OK;
 }
 
 }  // namespace

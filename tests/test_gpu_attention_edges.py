@@ -117,3 +117,22 @@ def test_strides_of_dimensions_of_one_do_not_matter(dev):
     done = torch.ones(2, dtype=torch.bool, device=dev)
     held = torch.zeros(2, 2, dtype=torch.int32, device=dev).as_strided((2, 1), (2, 5))
     assert paging.release_pages(ring, plans[0].free_state, held, new, done, page_size=16).tolist() == [2, 6, 0]
+
+
+def test_more_tokens_than_one_grid_has_blocks(dev):
+    """A grid has fewer than 2^32 threads: 2^24 blocks of 256, of a token each, are more than one launch."""
+    t, spec = (1 << 24) + 5, rotary.RotarySpec(2)
+    some = torch.tensor([0, 1, 77, t // 2, (1 << 24) - 2, (1 << 24) - 1, 1 << 24, t - 2, t - 1], device=dev)
+    x = torch.empty(t, 1, 130, device=dev, dtype=torch.bfloat16).normal_()
+    pos = torch.arange(t, device=dev, dtype=torch.int32) % 1000
+    y = rotary.apply_rotary(x, pos, spec)
+    assert torch.equal(y[some], rotary.apply_rotary(x[some], pos[some], spec))
+    del y
+    k = x.view(-1)[: t * 64].view(t, 1, 64)
+    cache, few = (kv4.KV4Cache(layers=1, kv_heads=1, head_dim=64, pages=n, page_size=256, device=dev) for n in ((t + 255) // 256, 1))
+    spec = rotary.RotarySpec(64)
+    kv4.append(cache, 0, k, k, torch.arange(t, device=dev), positions=pos, rotary=spec)
+    at = torch.arange(len(some), device=dev)
+    kv4.append(few, 0, k[some], k[some], at, positions=pos[some], rotary=spec)
+    for got, want in zip(kv4.read(cache, 0, some), kv4.read(few, 0, at)):
+        assert torch.equal(got, want)
