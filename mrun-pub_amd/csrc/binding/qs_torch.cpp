@@ -8,13 +8,16 @@
 
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/InferenceMode.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
 #include <map>
+#include <optional>
 #include <stdexcept>
 #include <string>
 #include <utility>
@@ -93,9 +96,19 @@ struct Device {
     REFUSE(index >= 0 && i != index, "QStore HIP operator tensors must share one device");
     index = i;
   }
+  c10::Device place() const { return c10::Device(c10::kCUDA, index); }
+  // The default stream is a null handle, which means the current device's: calls run under a guard.
   void* stream() const { return c10::hip::getCurrentHIPStream(index).stream(); }
   at::Tensor empty(at::IntArrayRef size, at::ScalarType type) const {
-    return at::detail::empty_cuda(size, type, c10::Device(c10::kCUDA, index), std::nullopt);
+    return at::detail::empty_cuda(size, type, place(), std::nullopt);
+  }
+};
+
+// Makes the tensors' device the current one for a call, if it is not already.
+struct Here {
+  std::optional<c10::DeviceGuard> guard;
+  explicit Here(const Device& d) {
+    if (c10::hip::current_device() != d.index) guard.emplace(d.place());
   }
 };
 
@@ -218,6 +231,7 @@ PyObject* plan_step(PyObject*, PyObject* const* v, Py_ssize_t n) {
     REFUSE(T < 0, "tokens must not be negative");
     Device d;
     d.add(ring), d.add(state), d.add(tables), d.add(past), d.add(fresh);
+    const Here here(d);
     // one allocation: slots and state in int64, then the rest in int32
     const at::Tensor all = d.empty({T + 3 + T + B + 1}, at::kLong);
     const int64_t words = 2 * (T + 3);
@@ -251,6 +265,7 @@ PyObject* rotary(PyObject*, PyObject* const* v, Py_ssize_t n) {
     const at::Tensor pos = positions_of(tensor(v[1], "positions"), T);
     Device d;
     d.add(x), d.add(pos);
+    const Here here(d);
     at::Tensor out;
     if (v[7] == Py_None) {
       out = d.empty({T, H, D}, x.scalar_type());
@@ -292,6 +307,7 @@ PyObject* append(PyObject*, PyObject* const* v, Py_ssize_t n) {
     Device d;
     d.add(k), d.add(val), d.add(slots), d.add(cache.storage);
     if (has_q) d.add(q);
+    const Here here(d);
     at::Tensor pos, freq, out;
     if (has_pos) d.add(tensor(v[6], "positions"));
     REFUSE(turns != has_pos, "rotary positions need both a spec and positions");
@@ -338,6 +354,7 @@ PyObject* read(PyObject*, PyObject* const* v, Py_ssize_t n) {
     uint8_t* base = cache.layer(v[1]);
     Device d;
     d.add(slots), d.add(cache.storage);
+    const Here here(d);
     const auto type = code == QS_F32 ? at::kFloat : code == QS_BF16 ? at::kBFloat16 : at::kHalf;
     at::Tensor k = d.empty({count, cache.kv_heads, cache.head_dim}, type), val = d.empty({count, cache.kv_heads, cache.head_dim}, type);
     check(entry.read(base, cache.pages, cache.page_size, (int)cache.kv_heads, (int)cache.head_dim,
@@ -380,6 +397,7 @@ PyObject* attend(PyObject*, PyObject* const* v, Py_ssize_t n) {
     uint8_t* base = cache.layer(v[2]);
     Device d;
     d.add(q), d.add(cache.storage), d.add(tables), d.add(starts), d.add(ctx);
+    const Here here(d);
     if (v[10] == Py_None) {
       out = d.empty({T, Hq, D}, q.scalar_type());
     } else {

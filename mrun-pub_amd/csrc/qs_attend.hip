@@ -20,6 +20,7 @@
 //   4095 tokens, 32 + 8 heads                188 us  731 TFLOP/s (171, 801): vector operations 49% and
 //                                                    products 38% of the cycles, hardly at once
 //   chunks of 701, window 1024, fp32 of 64  36.1 us  153 TFLOP/s, the fp32 product's own rate
+#include <atomic>
 #include <type_traits>
 
 #include "qs_kv4.h"
@@ -1452,9 +1453,17 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
       a.least = kRowsLeast;
       a.whole = kRowsWhole;
       const size_t lds = 2 * sizeof(RowsTile<T, D>);
-      static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attend_rows<T, D>),
-                                                            hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-      if (allowed != hipSuccess) return hip_check(allowed, "k_attend_rows shared memory");
+      static std::atomic<uint64_t> allowed{0};  // a bit a device
+      int device = 0;
+      int status = hip_check(hipGetDevice(&device), "k_attend_rows device");
+      if (status != QS_OK) return status;
+      if (!(allowed.load(std::memory_order_relaxed) >> (device & 63) & 1)) {
+        status = hip_check(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_attend_rows<T, D>),
+                                               hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
+                           "k_attend_rows shared memory");
+        if (status != QS_OK) return status;
+        allowed.fetch_or(uint64_t(1) << (device & 63), std::memory_order_relaxed);
+      }
       hipLaunchKernelGGL((k_attend_rows<T, D>), dim3((unsigned)p.grid_rows), dim3(256), lds, s, a.starts, a.context, a.T,
                        a.B, a.Hkv, a.grp, a.reach, a.window, a.blocks, a);
     }

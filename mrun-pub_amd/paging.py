@@ -95,9 +95,10 @@ def release_pages(
         raise ValueError("done must be a bool vector of one value per request")
     device = nat.require_device(ring, free_state, block_tables, held, done)
     state = torch.empty(3, dtype=torch.int64, device=device)
-    nat.call(
-        "qs_release_pages", nat.ptr(ring), int(ring.numel()), nat.ptr(free_state), nat.ptr(state),
-        nat.ptr(block_tables), block_tables.stride(0), int(block_tables.shape[1]), nat.ptr(held),
-        nat.ptr(done.contiguous()), B, int(page_size), nat.stream_of(device),
-    )
+    with torch.cuda.device(device):  # the default stream's handle means the current device's
+        nat.call(
+            "qs_release_pages", nat.ptr(ring), int(ring.numel()), nat.ptr(free_state), nat.ptr(state),
+            nat.ptr(block_tables), block_tables.stride(0), int(block_tables.shape[1]), nat.ptr(held),
+            nat.ptr(done.contiguous()), B, int(page_size), nat.stream_of(device),
+        )
     return state

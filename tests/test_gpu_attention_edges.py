@@ -136,3 +136,25 @@ def test_more_tokens_than_one_grid_has_blocks(dev):
     kv4.append(few, 0, k[some], k[some], at, positions=pos[some], rotary=spec)
     for got, want in zip(kv4.read(cache, 0, some), kv4.read(few, 0, at)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_tensors_of_another_device_than_the_current_one(dev):
+    """Calls run on their tensors' device, on its current stream, whatever the current device is; a tile
+    of 68 KB of LDS (fp32 prompts, heads of 128) is allowed on each."""
+    outs = []
+    for at in (torch.device("cuda:0"), torch.device("cuda:1")):
+        with torch.cuda.device(0):
+            s = Setup(dev, [300, 40], [200, 1], 4, 2, 128, 16, torch.float32, seed=1)
+            cache = kv4.KV4Cache(layers=1, kv_heads=2, head_dim=128, pages=s.cache.pages, page_size=16, device=at)
+            k, v, slots = s.k.to(at), s.v.to(at), torch.tensor(np.concatenate(s.slots), device=at)
+            spec, pos = rotary.RotarySpec(128), torch.arange(340, device=at)
+            kv4.append(cache, 0, rotary.apply_rotary(k, pos, spec), v, slots)
+            out = kv4.attend(s.q.to(at), cache, 0, s.tables.to(at), i32(s.starts, at), i32(s.ctx, at), max_query=200)
+            ring, state = paging.free_pages(8, at)
+            p = paging.plan_step(ring, state, torch.full((1, 4), -1, dtype=torch.int32, device=at), i32([0], at), i32([9], at),
+                                 page_size=16, tokens=9)
+            freed = paging.release_pages(ring, p.free_state, torch.zeros(1, 4, dtype=torch.int32, device=at), i32([9], at),
+                                         torch.ones(1, dtype=torch.bool, device=at), page_size=16)
+            outs.append([x.cpu() for x in (out, *kv4.read(cache, 0, slots), *p, freed)])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
