@@ -470,7 +470,8 @@ struct QueryRow {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sums[k * STRIDE / kKv4Group] += v[k][e];
     }
-    return __builtin_amdgcn_ldexpf(scale_log2, e2);
+    // neither 0 nor infinite, either of which would make NaN of a score: hidden ones are -inf, others may be 0
+    return __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(scale_log2, e2), 0x1p-126f, 0x1.fffffep127f);
   }
 };
 

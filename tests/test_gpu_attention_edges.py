@@ -138,6 +138,20 @@ def test_more_tokens_than_one_grid_has_blocks(dev):
         assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("dtype,size,scale", [(torch.bfloat16, 1e-30, 1e-30), (torch.bfloat16, 2.0**-133, 1e-45),
+                                              (torch.float16, 2.0**-24, 1e-45), (torch.float32, 1e-45, 1e-45),
+                                              (torch.bfloat16, 0.0, 3e38), (torch.float16, 0.0, 3e38), (torch.float32, 0.0, 3e38)])
+@pytest.mark.parametrize("new", [1, 40])
+def test_scores_of_zero_weigh_all_tokens_alike(dev, new, dtype, size, scale):
+    """Scores that are zero or far below a weight's step, from tiny queries and scales or from zeros at
+    the largest scale: every visible token has the same weight, and hidden ones none."""
+    s = Setup(dev, [77], [new], 8, 2, 64, 16, dtype, seed=new)
+    s.q = torch.full_like(s.q, size)
+    out = s.attend(scale=scale)
+    s.q.zero_()
+    s.check(out)
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_tensors_of_another_device_than_the_current_one(dev):
     """Calls run on their tensors' device, on its current stream, whatever the current device is; a tile
