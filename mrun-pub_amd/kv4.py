@@ -10,6 +10,8 @@ token's key of 128 values, against 256 in 16 bits.  NaN is stored as 0 and value
   turns queries and keys by their rotary positions on the way;
 * ``attend`` is attention of the step's queries over the cache, the step's own tokens included;
 * ``read`` gives back what slots hold.
+
+They are for serving: results are inference tensors, and no gradient goes through them.
 """
 
 from __future__ import annotations

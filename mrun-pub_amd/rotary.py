@@ -91,6 +91,23 @@ class RotarySpec:
         return f
 
 
+class _Turn(torch.autograd.Function):
+    """The turn as autograd sees it: linear in x, with the inverse turn as its gradient."""
+
+    @staticmethod
+    def forward(ctx, x, positions, spec, inverse):
+        # what a step's plan gave is an inference tensor, which autograd keeps no hold of
+        ctx.save_for_backward(positions.clone() if positions.is_inference() else positions)
+        ctx.spec, ctx.inverse = spec, inverse
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)  # the binding's own would be an inference tensor
+        return nat.fast().rotary(x, positions, spec.on(x.device), spec.dim, spec.interleaved, inverse, spec.magnitude, out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        (positions,) = ctx.saved_tensors
+        return apply_rotary(grad, positions, ctx.spec, inverse=not ctx.inverse), None, None, None
+
+
 def apply_rotary(
     x: torch.Tensor, positions: torch.Tensor, spec: RotarySpec, *, inverse: bool = False,
     out: torch.Tensor | None = None,
@@ -100,7 +117,15 @@ def apply_rotary(
 
     ``x`` may be any view whose last dimension is contiguous (a slice of a fused projection).
     ``inverse=True`` turns back, which is also the gradient: with respect to x, of a loss whose
-    gradient with respect to the result is given.  ``out`` may be ``x`` itself.
+    gradient with respect to the result is given.  Where ``x`` requires a gradient autograd takes it
+    so; otherwise the result is an inference tensor, as every operator's here.  ``out`` may be ``x``
+    itself; it takes no gradient.
     """
+    if x.requires_grad and torch.is_grad_enabled():
+        if out is not None:
+            raise ValueError("rotary output given by out= takes no gradient, and x requires one")
+        if not x.is_cuda:
+            raise ValueError("QStore HIP operators require tensors on a HIP (cuda) device")
+        return _Turn.apply(x, positions, spec, inverse)
     freq = spec.on(x.device) if x.is_cuda else None
     return nat.fast().rotary(x, positions, freq, spec.dim, spec.interleaved, inverse, spec.magnitude, out)

@@ -152,6 +152,29 @@ def test_scores_of_zero_weigh_all_tokens_alike(dev, new, dtype, size, scale):
     s.check(out)
 
 
+@pytest.mark.parametrize("layout", rotary.LAYOUTS)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_autograd_takes_the_inverse_turn_as_the_gradient(dev, layout, dtype):
+    spec = rotary.RotarySpec(32, layout=layout, scaling={"type": "yarn", "factor": 4.0, "original": 64})
+    x, g = (torch.randn(5, 3, 48, device=dev).to(dtype) for _ in range(2))
+    pos = paging.plan_step(*paging.free_pages(4, dev), torch.zeros(1, 4, dtype=torch.int32, device=dev), i32([7], dev), i32([5], dev),
+                           page_size=16, tokens=5).positions  # an inference tensor
+    back = rotary.apply_rotary(g, pos, spec, inverse=True)
+    for inverse, want in ((False, back), (True, rotary.apply_rotary(g, pos, spec))):
+        leaf = x.clone().requires_grad_()
+        y = rotary.apply_rotary(leaf * 2, pos, spec, inverse=inverse)
+        assert torch.equal(y.detach(), rotary.apply_rotary(x * 2, pos, spec, inverse=inverse))
+        y.backward(g)
+        assert torch.equal(leaf.grad, want * 2)
+    leaf = x.clone().requires_grad_()
+    (wide,) = torch.autograd.grad(rotary.apply_rotary(leaf, pos, spec).sum(), leaf)  # a broadcast gradient
+    assert torch.equal(wide, rotary.apply_rotary(torch.ones_like(x), pos, spec, inverse=True))
+    with torch.no_grad():
+        assert not rotary.apply_rotary(leaf, pos, spec).requires_grad
+    with pytest.raises(ValueError, match="gradient"):
+        rotary.apply_rotary(leaf, pos, spec, out=torch.empty_like(x))
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_tensors_of_another_device_than_the_current_one(dev):
     """Calls run on their tensors' device, on its current stream, whatever the current device is; a tile
