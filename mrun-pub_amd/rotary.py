@@ -83,9 +83,12 @@ class RotarySpec:
         return plain / factor * ramp + plain * (1.0 - ramp)
 
     def on(self, device: torch.device) -> torch.Tensor:
-        """The fp64 frequencies on ``device``."""
+        """The fp64 frequencies on ``device``, laid out there by the first call, which a graph does not
+        capture: a program that captures its steps calls this (or a step) before."""
         f = self._on.get(device)
         if f is None:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("rotary frequencies are not on the device yet: call spec.on(device) before the capture")
             f = self._on[device] = self.frequencies.to(device)
             torch.cuda.current_stream(device).synchronize()  # other streams may read it from now on
         return f

@@ -3,6 +3,9 @@
 from __future__ import annotations
 
 import pytest
+import torch
+
+from mrun_pub_amd import rotary
 
 FAKE = 1 << 20  # an aligned pointer that is never read: the checks come first
 
@@ -22,3 +25,10 @@ def test_attention_of_more_threads_than_a_grid_has(tokens, heads, kv_heads, dtyp
          None, 0, None]
     assert lib.qs_kv4_attend(*a) == nat.QS_ERR_LIMIT
     assert b"threads" in lib.qs_last_error()
+
+
+def test_rotary_frequencies_are_not_laid_out_in_a_capture(monkeypatch):
+    """The copy and the wait of the first use would end a graph's capture with an error of their own."""
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="before the capture"):
+        rotary.RotarySpec(64).on(torch.device("cuda:0"))
