@@ -8,7 +8,7 @@ import torch
 
 from mrun_pub_amd import kv4, paging, rotary
 from oracle import attention as oa
-from test_gpu_attention import Setup, f64, i32
+from test_gpu_attention import HALF, TINY, Setup, f64, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -173,6 +173,48 @@ def test_autograd_takes_the_inverse_turn_as_the_gradient(dev, layout, dtype):
         assert not rotary.apply_rotary(leaf, pos, spec).requires_grad
     with pytest.raises(ValueError, match="gradient"):
         rotary.apply_rotary(leaf, pos, spec, out=torch.empty_like(x))
+
+
+def sizes(x):
+    """Of cached values [n, h, d]: the largest code * s and |lo| that their groups' sums can hold, a value each."""
+    g = x.reshape(*x.shape[:-1], -1, 64)
+    top = (g.max(-1) - g.min(-1)) * 1.01 + abs(g).max(-1)  # codes 0 and 15 are not always there
+    return np.repeat(top, 64, -1)
+
+
+@pytest.mark.parametrize("hq,hkv,d,ctx,new", [(8, 2, 128, 3, 3), (4, 1, 64, 12, 1), (8, 2, 128, 20, 20), (4, 4, 64, 40, 40), (4, 1, 256, 9, 5),
+                                              (4, 1, 256, 33, 12)])
+def test_fp16_attention_multiplies_exact_codes(dev, hq, hkv, d, ctx, new):
+    """Queries of zero give the mean of the values: weights of 1, scales of 11 bits in two bf16 parts and
+    codes are exact, so fp16 results are off by their own rounding and by fp32 sums.  Values rounded to
+    fp16, or weights to one bf16 part, would be off by more."""
+    s = Setup(dev, [ctx], [new], hq, hkv, d, 16, torch.float16, seed=ctx + d)
+    out, v = f64(s.attend(torch.zeros_like(s.q))), s.values[0]
+    _, sc, lo = oa.kv4_quantize(v.astype(np.float32))
+    one = torch.tensor(sc.astype(np.float32)).bfloat16().double().numpy()  # a scale's first part
+    sc, lo, one = (np.repeat(x.astype(np.float64), 64, -1) for x in (sc, lo, one))
+    zero = np.zeros(s.q.shape)
+
+    def mean(x):
+        return oa.attend(zero, s.keys, [x], s.starts, s.ctx, 1.0)[0]
+
+    want, half = mean(v), HALF[torch.float16]
+    bound = half * abs(want) + (ctx + 8) * 2.0**-24 * mean(15 * sc + abs(lo)) + TINY[torch.float16]
+    assert (abs(out - want) <= bound).all()
+    for other in (v.astype(np.float16).astype(np.float64), (v - lo) * one / sc + lo):  # the bound tells these apart
+        assert (abs(mean(other) - want) > bound).any()
+
+
+@pytest.mark.parametrize("hq", [2, 80])
+def test_fp16_rows_that_see_one_token(dev, hq):
+    """They give its value rounded to fp16 once: a weight of 1 times a scale of 11 bits is exact in two parts."""
+    s = Setup(dev, [1, 300], [1, 300], hq, 2, 128, 16, torch.float16, seed=11)
+    out = f64(s.attend(window=1))
+    for b in range(2):
+        v = s.values[b][s.ctx[b] - s.new[b]:]
+        want, size = (np.repeat(x, hq // 2, 1) for x in (v, sizes(v)))
+        got = out[s.starts[b]: s.starts[b + 1]]
+        assert (abs(got - want) <= HALF[torch.float16] * abs(want) + 2.0**-23 * size + TINY[torch.float16]).all()
 
 
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
