@@ -205,6 +205,22 @@ def test_fp16_attention_multiplies_exact_codes(dev, hq, hkv, d, ctx, new):
         assert (abs(mean(other) - want) > bound).any()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ctx,new", [(8, 1), (8, 8), (40, 5), (40, 40), (300, 1), (300, 90)])
+def test_fp16_scores_use_exact_keys(dev, d, ctx, new):
+    """At a scale of 1 scores are large, and their errors show: in fp32 sums of terms of some 700 they are
+    about 2^-15, which beside the result's own rounding (0.29 of 2^-10 in the 2-norm) adds a hundredth
+    to it.  Keys rounded to fp16 would add more than half."""
+    s = Setup(dev, [ctx], [new], 8, 2, d, 16, torch.float16, seed=ctx + d)
+    out, q = f64(s.attend(scale=1.0)), f64(s.q)
+    want, _, _ = oa.attend(q, s.keys, s.values, s.starts, s.ctx, 1.0)
+    own = np.linalg.norm(want.astype(np.float16) - want)
+    assert np.linalg.norm(out - want) <= 1.1 * own
+    if new > 1:  # one token's rows are too few for the norms to tell
+        other, _, _ = oa.attend(q, [s.keys[0].astype(np.float16).astype(np.float64)], s.values, s.starts, s.ctx, 1.0)
+        assert np.linalg.norm(other.astype(np.float16) - want) > 1.5 * own
+
+
 @pytest.mark.parametrize("hq", [2, 80])
 def test_fp16_rows_that_see_one_token(dev, hq):
     """They give its value rounded to fp16 once: a weight of 1 times a scale of 11 bits is exact in two parts."""
