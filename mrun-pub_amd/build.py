@@ -1,5 +1,7 @@
 """Build ``libqstore_hip.so`` (the gfx950 kernels + C ABI) in-tree with hipcc, and ``_qs_torch.so``
-(host code: the torch binding of the operators whose calls have to be short) with g++.
+(host code: the torch binding of the operators whose calls have to be short) with g++, or with
+hipcc where there is none.  The kernels' library does not wait for the binding: it is built, and
+serves every other operator, also where the binding fails, which is raised at the end.
 
 Usage: ``python mrun-pub_amd/build.py`` or ``build()`` from Python.  Objects go to
 ``mrun-pub_amd/_build/``; the shared library lands next to this file so it travels
@@ -93,7 +95,7 @@ def _build_binding() -> Path:
     home, out = Path(torch.__file__).resolve().parent, PKG_DIR / BINDING_NAME
     tmp = out.with_suffix(".so.tmp")
     cmd = [
-        os.environ.get("CXX", "g++"), "-O2", "-fPIC", "-shared", "-std=c++17", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        os.environ.get("CXX") or shutil.which("g++") or HIPCC, "-O2", "-fPIC", "-shared", "-std=c++17", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", str(home / "include"), "-isystem",
         str(home / "include/torch/csrc/api/include"), "-isystem", str(Path(HIPCC).resolve().parent.parent / "include"),
         "-isystem", sysconfig.get_paths()["include"], str(CSRC / "binding" / "qs_torch.cpp"), "-o", str(tmp),
@@ -107,7 +109,8 @@ def _build_binding() -> Path:
 
 
 def build(verbose: bool = False) -> Path:
-    """Compile every HIP/C++ source and link the libraries; returns the kernels' path."""
+    """Compile every HIP/C++ source and link the libraries; returns the kernels' path.  A binding that
+    does not build is raised after the kernels' library is in place."""
     if not Path(HIPCC).exists() and shutil.which("hipcc") is None:
         raise RuntimeError("hipcc not found: the QStore HIP library cannot be built")
     BUILD_DIR.mkdir(exist_ok=True)
@@ -115,13 +118,13 @@ def build(verbose: bool = False) -> Path:
     with ThreadPoolExecutor(max_workers=min(8, len(sources) + 1)) as pool:
         binding = pool.submit(_build_binding)
         objs = list(pool.map(_compile, sources))
-        binding.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(tmp), *map(str, objs)]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"link failed:\n{proc.stderr}")
     os.replace(tmp, LIB_PATH)
+    binding.result()
     if verbose:
         print(f"built {LIB_PATH} from {len(sources)} sources")
     return LIB_PATH
