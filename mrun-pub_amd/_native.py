@@ -193,7 +193,7 @@ _FAST = ("qs_plan_step", "qs_rotary", "qs_kv4_append", "qs_kv4_read", "qs_kv4_at
 
 def fast():
     """The binding module of the operators whose calls have to be short (checks, allocations and the
-    launch in one native call).  Raises RuntimeError if it is not built."""
+    launch in one native call).  Raises RuntimeError if it is not built, or built for another torch."""
     global _fast
     if _fast is None:
         lib = load()
@@ -201,6 +201,9 @@ def fast():
             from . import _qs_torch as module
         except ImportError as exc:
             raise RuntimeError("QStore torch binding not built; run __graft_entry__.build()") from exc
+        if module.built_for != torch.__version__:
+            raise RuntimeError(f"QStore torch binding built for torch {module.built_for}, not {torch.__version__}; "
+                               "run __graft_entry__.build()")
         module.bind(*(ctypes.cast(getattr(lib, name), _P).value for name in _FAST))
         _fast = module
     return _fast

@@ -96,6 +96,7 @@ def _build_binding() -> Path:
     tmp = out.with_suffix(".so.tmp")
     cmd = [
         os.environ.get("CXX") or shutil.which("g++") or HIPCC, "-O2", "-fPIC", "-shared", "-std=c++17", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        f'-DQS_BUILT_FOR="{torch.__version__}"',
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-isystem", str(home / "include"), "-isystem",
         str(home / "include/torch/csrc/api/include"), "-isystem", str(Path(HIPCC).resolve().parent.parent / "include"),
         "-isystem", sysconfig.get_paths()["include"], str(CSRC / "binding" / "qs_torch.cpp"), "-o", str(tmp),

@@ -445,4 +445,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_qs_torch", nullptr, -1, methods, 
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__qs_torch() { return PyModule_Create(&module); }
+// built_for: the torch whose C++ interface this was compiled against, which no other need have.
+PyMODINIT_FUNC PyInit__qs_torch() {
+  PyObject* m = PyModule_Create(&module);
+  if (m && PyModule_AddStringConstant(m, "built_for", QS_BUILT_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

@@ -47,3 +47,17 @@ def test_the_binding_is_built_without_gxx(build, monkeypatch):
     with pytest.raises(RuntimeError, match="not run"):
         build._build_binding()
     assert [c[0] for c in commands] == [build.HIPCC]
+
+
+def test_a_binding_of_another_torch_is_refused(monkeypatch):
+    import torch
+
+    from mrun_pub_amd import _native as nat
+
+    if not nat.LIB_PATH.exists():
+        pytest.skip("library not built")
+    assert nat.fast() is nat.fast()
+    monkeypatch.setattr(nat, "_fast", None)
+    monkeypatch.setattr(torch, "__version__", "1.0")
+    with pytest.raises(RuntimeError, match="not 1.0"):
+        nat.fast()
