@@ -43,9 +43,10 @@ struct AttendArgs {
   const int* starts;
   const int* context;
   void* out;
-  float* part_o;    // [block][rows of a tile * D]
-  float2* part_ml;  // [block][rows of a tile]
-  int* done;        // [block]: parts finished of the tile whose first block it is; 0 between calls
+  // places: `blocks` of them, for the parts of tiles that are cut into several
+  float* part_o;    // [place][rows of a tile * D]
+  float2* part_ml;  // [place][rows of a tile]
+  int* done;        // [place]: parts finished of the tile whose first part's it is; 0 between calls
   int64_t ldq_t, ldq_h, ld_table;
   int pages, P, shift, Hkv, grp, T, B, window;
   int reach;                // tokens that a table row has room for, 2^30 at most
@@ -227,7 +228,7 @@ struct Work {
   int64_t q0;         // first token of the request
   int b, n, ctx, row0;  // request, its new tokens and context, first row of the tile
   int part, parts;    // which part of the tile's tokens, of how many
-  int64_t first;      // block of the tile's part 0
+  int64_t first;      // place of the tile's part 0 (of one KV head's, as are blocks)
   int hk;
   bool any;
 };
@@ -303,8 +304,11 @@ __device__ __forceinline__ int wave_scan(int v) {
 
 // With parts: a tile whose tokens take W steps is cut into ceil(W / size) parts, size so that all
 // requests' tiles and parts come to at most a.blocks blocks, which run at once, if the tiles alone
-// do not pass that.  Every block does the sums over the requests itself: up to 63 requests each of
-// its waves, a lane a request; more with all its threads, and LDS between the waves.
+// do not pass that.  The parts of tiles that are cut come to no more in any case, so they have places
+// of their own and tiles that are not cut need none: 34 MB hold the parts of prompts of heads of 128,
+// where a place a block took 103 MB for a prompt of 4095 and more for longer ones.
+// Every block does the sums over the requests itself: up to 63 requests each of its waves, a lane a
+// request; more with all its threads, and LDS between the waves.
 template <int R, int STEP, int THREADS>
 __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_sum, Work* s_work) {
   constexpr int NW = THREADS / 64;
@@ -348,30 +352,51 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
   const float total = total_of(sum);
   float size = total * 1.00001f / most + 1.f;  // sums of rounded products: never too small
   if (size < (float)a.least) size = (float)a.least;
-  int count = 0;
+  int count, before, place;
 #pragma unroll 1
   for (int round = 0;; ++round) {
+    int cut = 0;  // blocks of tiles with several parts, of this thread's
     count = 0;
     for (int b = b0; b < b1; ++b) {
       if (each > 1) look(b);
-      count += tiles * parts_for(1.f / size);
+      const int parts = parts_for(1.f / size);
+      count += tiles * parts;
+      cut += parts > 1 ? tiles * parts : 0;
     }
-    if (round == 3) break;
-    const float all = total_of((float)count);
-    if (all <= most) break;
-    // what rounding up adds to total / size parts changes little with the size
-    const float room = most - (all - total / size);
-    size = room > 0.5f * total / size ? total * 1.001f / room : 2.f * size;
+    if (round < 3) {
+      const float all = total_of((float)count);
+      if (all > most) {
+        // what rounding up adds to total / size parts changes little with the size
+        const float room = most - (all - total / size);
+        size = room > 0.5f * total / size ? total * 1.001f / room : 2.f * size;
+        continue;
+      }
+      round = 3;
+    }
+    // Blocks and places before this thread's, in one sum: both are below 2^15, the tiles' bound of
+    // 4 a.blocks (plan_grid) and a block more for each part.
+    const int both = count | cut << 16;
+    int sum = wave_scan(both), all = __builtin_amdgcn_readlane(sum, 63);
+    sum -= both;
+    if (!alone) {
+      __syncthreads();
+      if (lane == 0) s_sum[wave] = __int_as_float(all);
+      if (threadIdx.x == 0) s_work->any = false;
+      __syncthreads();
+      all = 0;
+#pragma unroll 1
+      for (int w = 0; w < NW; ++w) {
+        const int other = __float_as_int(s_sum[w]);
+        if (w < wave) sum += other;
+        all += other;
+      }
+    }
+    before = sum & 0xffff;
+    place = sum >> 16;
+    if ((float)(all >> 16) <= most) break;
+    size *= 1.25f;  // no tile is cut at the latest where this passes its steps
   }
   const float per_step = 1.f / size;
-  int before = wave_scan(count) - count;
-  if (!alone) {
-    __syncthreads();
-    if (lane == 63) s_sum[wave] = __int_as_float(before + count);
-    if (threadIdx.x == 0) s_work->any = false;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) before += __float_as_int(s_sum[w]);
-  }
   Work t;
   const bool found = y >= before && y < before + count;
   if (alone) {
@@ -386,11 +411,13 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
     t.n = __builtin_amdgcn_readlane(n, from);
     t.ctx = __builtin_amdgcn_readlane(ctx, from);
     before = __builtin_amdgcn_readlane(before, from);
+    place = __builtin_amdgcn_readlane(place, from);
     tiles = __builtin_amdgcn_readlane(tiles, from);
     t.parts = __builtin_amdgcn_readlane(parts_for(per_step), from);
     const int tile = (y - before) / t.parts;
     t.row0 = (tiles - 1 - tile) * R;
     t.part = y - before - tile * t.parts;
+    t.first = place + tile * t.parts;
     t.any = true;
   } else {
     if (found) {
@@ -406,17 +433,18 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
           t.row0 = (tiles - 1 - tile) * R;
           t.part = y - before - tile * parts;
           t.parts = parts;
+          t.first = place + tile * parts;
           t.any = true;
           *s_work = t;
           break;
         }
         before += tiles * parts;
+        if (parts > 1) place += tiles * parts;
       }
     }
     __syncthreads();
     t = *s_work;
   }
-  t.first = y - t.part;
   return t;
 }
 
@@ -1390,7 +1418,7 @@ __global__ __launch_bounds__(256, D == 256 || (kKind<T> == 2 && D == 128) ? 1 : 
 
 // ---- launch -------------------------------------------------------------------------------
 constexpr int kFewRows = 32;
-constexpr int kSyncWords = 8192;  // of the workspace's start, one a block
+constexpr int kSyncWords = 8192;  // of the workspace's start, one a place: at most 1024 blocks run at once
 
 struct Plan {
   int rt;           // 16-row tiles of k_attend_few, 0: not used
@@ -1408,7 +1436,7 @@ void plan_grid(int64_t T, int64_t B, int Hkv, int grp, int R, int64_t rows, int6
   const int64_t tiles = (T * grp / R + B + 1) * Hkv;
   const int64_t likely = cdiv(rows, R) * B * Hkv * cdiv(steps, least);
   fill = steps > whole && tiles <= 4 * most && B < 1024 ? (int)(likely < most ? likely : most) : 0;
-  if (tiles + fill + Hkv > kSyncWords) fill = 0;
+  if (fill < Hkv) fill = 0;  // not a part a head
   grid = tiles + (fill ? fill + Hkv : 0);
 }
 
@@ -1436,8 +1464,8 @@ Plan plan_of(int kind, int D, int64_t T, int64_t B, int Hkv, int grp, int64_t ma
 }
 
 size_t space_of(const Plan& p, int D) {  // the kernels' parts, which run one after the other
-  const size_t few = p.rt && p.fill_few ? (size_t)p.grid_few * 16 * p.rt : 0;
-  const size_t rows = p.rows && p.fill_rows ? (size_t)p.grid_rows * 128 : 0;
+  const size_t few = p.rt ? (size_t)p.fill_few * 16 * p.rt : 0;
+  const size_t rows = p.rows ? (size_t)p.fill_rows * 128 : 0;
   const size_t most = few > rows ? few : rows;
   return most ? (kSyncWords + most * (D + 2)) * sizeof(float) : 0;
 }
@@ -1447,7 +1475,7 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
   constexpr bool wide = kKind<T> == 2 && D == 256;
   if constexpr (!wide)
     if (p.rows) {
-      a.part_ml = reinterpret_cast<float2*>(a.part_o + p.grid_rows * 128 * D);
+      a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)p.fill_rows * 128 * D);
       a.rows_from = p.rt ? kFewRows + 1 : 0;
       a.rows_upto = 0x7fffffff;
       a.blocks = p.fill_rows;
@@ -1469,7 +1497,7 @@ int launch_attend(AttendArgs a, const Plan& p, hipStream_t s) {
                        a.B, a.Hkv, a.grp, a.reach, a.window, a.blocks, a);
     }
   if (p.rt) {
-    a.part_ml = reinterpret_cast<float2*>(a.part_o + p.grid_few * 16 * p.rt * D);
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)p.fill_few * 16 * p.rt * D);
     a.rows_from = 0;
     a.rows_upto = p.rows ? kFewRows : 0x7fffffff;
     a.blocks = p.fill_few;

@@ -32,3 +32,16 @@ def test_rotary_frequencies_are_not_laid_out_in_a_capture(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     with pytest.raises(RuntimeError, match="before the capture"):
         rotary.RotarySpec(64).on(torch.device("cuda:0"))
+
+
+@pytest.mark.parametrize("tokens,requests,kv_heads,heads,d,new,context", [
+    (4095, 1, 8, 32, 128, 4095, 4095), (8000, 1, 8, 32, 128, 8000, 8000), (2048, 4, 8, 32, 128, 512, 30000),
+    (4095, 1, 8, 32, 256, 4095, 4095), (64, 64, 8, 32, 128, 1, 131072), (320, 64, 8, 32, 256, 5, 131072), (1, 1, 2, 12, 128, 1, 131072),
+])
+def test_attention_workspace_holds_cut_tiles_alone(tokens, requests, kv_heads, heads, d, new, context):
+    """A place a block that runs at once, 512 of 128 rows or 1024 of 16, each its rows' sums, maxima and
+    totals in fp32: whatever the number of tiles.  (Two tiles of 16 rows a block: half as many run.)"""
+    _nat, lib = _lib()
+    size = lib.qs_kv4_attend_workspace_bytes(tokens, requests, kv_heads, heads, d, 64, new, context, 0)
+    rows = 512 * 128 if new * heads // kv_heads > 32 else 1024 * 16
+    assert 0 < size <= 4 * (8192 + rows * (d + 2))

@@ -233,6 +233,30 @@ def test_fp16_rows_that_see_one_token(dev, hq):
         assert (abs(got - want) <= HALF[torch.float16] * abs(want) + 2.0**-23 * size + TINY[torch.float16]).all()
 
 
+@pytest.mark.parametrize("groups", [((4, 1280, 5300), (6, 1280, 1280)), ((40, 128, 5300), (60, 128, 1280)), ((3, 1000, 9000), (1, 3000, 3000))])
+def test_more_parts_than_places(dev, groups):
+    """Prompts of unequal contexts whose tiles alone are more than the blocks that run at once: cut tiles
+    have a place for each part or are cut less.  Results as without parts, each off by the roundings of
+    sums over its tokens."""
+    new, ctx = (sum(([g[i]] * g[0] for g in groups), []) for i in (1, 2))
+    d, P = 64, 64
+    count = [-(-c // P) for c in ctx]
+    cache = kv4.KV4Cache(layers=1, kv_heads=8, head_dim=d, pages=sum(count), page_size=P, device=dev)
+    tables = torch.full((len(ctx), max(count)), -1, dtype=torch.int32, device=dev)
+    order, at = torch.randperm(sum(count), device=dev).int(), 0
+    for b, n in enumerate(count):
+        tables[b, :n] = order[at: at + n]
+        at += n
+    k, v = (torch.randn(cache.pages * P, 8, d, device=dev) for _ in range(2))
+    kv4.append(cache, 0, k, v, torch.arange(cache.pages * P, device=dev))
+    q = torch.randn(sum(new), 8, d, device=dev)
+    args = (q, cache, 0, tables, i32(np.cumsum([0] + new), dev), i32(ctx, dev))
+    want = kv4.attend(*args, max_query=max(new), max_context=1).double()  # no parts
+    for _ in range(2):
+        got = kv4.attend(*args, max_query=max(new), max_context=max(ctx))
+        assert float((got - want).norm() / want.norm()) <= 2 * (max(ctx) / 16) ** 0.5 * 2.0**-24
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_tensors_of_another_device_than_the_current_one(dev):
     """Calls run on their tensors' device, on its current stream, whatever the current device is; a tile
