@@ -1430,14 +1430,17 @@ struct Plan {
 
 // Blocks of one kernel, R rows a tile: a block a tile and head, and with parts `fill` more, if by the
 // caller's bounds some tile has more steps than stay whole.  Tiles in thousands fill the chip without
-// parts, and the sums over many requests would cost every block more.
-void plan_grid(int64_t T, int64_t B, int Hkv, int grp, int R, int64_t rows, int64_t steps, int whole, int least, int most,
-               int64_t& grid, int& fill) {
-  const int64_t tiles = (T * grp / R + B + 1) * Hkv;
+// parts, and the sums over many requests would cost every block more.  upto: rows of the requests that
+// are this kernel's, whose tiles then are bounded by the requests (without parts a tile's block is
+// found by the tokens before it, so those of every request count).
+void plan_grid(int64_t T, int64_t B, int Hkv, int grp, int R, int64_t rows, int64_t upto, int64_t steps, int whole, int least,
+               int most, int64_t& grid, int& fill) {
+  const int64_t all = T * grp / R + B + 1, own = (B + 1) * cdiv(upto, R);
+  const int64_t tiles = (own < all ? own : all) * Hkv;
   const int64_t likely = cdiv(rows, R) * B * Hkv * cdiv(steps, least);
   fill = steps > whole && tiles <= 4 * most && B < 1024 ? (int)(likely < most ? likely : most) : 0;
   if (fill < Hkv) fill = 0;  // not a part a head
-  grid = tiles + (fill ? fill + Hkv : 0);
+  grid = fill ? tiles + fill + Hkv : all * Hkv;
 }
 
 Plan plan_of(int kind, int D, int64_t T, int64_t B, int Hkv, int grp, int64_t max_query, int64_t max_context, int64_t window) {
@@ -1452,13 +1455,17 @@ Plan plan_of(int kind, int D, int64_t T, int64_t B, int Hkv, int grp, int64_t ma
   const int64_t steps = cdiv(span, 32), tiles = (T * grp / (16 * p.rt) + B + 1) * Hkv;
   p.form = few_form(kind, D, p.rt, B * Hkv * steps <= 8192, B * Hkv <= 64, tiles > 256 && steps <= 8);
   const int most = few_fill(kind, D, p.rt, p.form);
-  // the tiles of a few requests' few rows find room beside the others; a launch of their own costs more
-  if (p.rows && B * Hkv <= 128) p.rt = 0;
+  // The tiles of a few requests' few rows find room beside the others, unless their contexts are long:
+  // a block of 128 rows reads a context no faster for 4 of them.  32 + 8 heads, one launch and two: 15
+  // tokens over 2000 beside a prompt of 500 31 and 42 us, over 4000 45 and 48, over 8000 75 and 62, over
+  // 16000 140 and 83; 31 over 2000 (256 heads) 58 and 49; 3 over 131072 beside 4000 1682 and 277; and where
+  // no request has few rows, 4 chunks of 512 over 4000 153 and 160, over 16000 574 and 574.
+  if (p.rows && B * Hkv <= 128 && (B == 1 || span <= 4096)) p.rt = 0;
   if (p.rt)
-    plan_grid(T, B, Hkv, grp, 16 * p.rt, rows < kFewRows ? rows : kFewRows, cdiv(span, 32) + 1, kFewWhole, kFewLeast, most,
-              p.grid_few, p.fill_few);
+    plan_grid(T, B, Hkv, grp, 16 * p.rt, rows < kFewRows ? rows : kFewRows, p.rows ? kFewRows : INT32_MAX, cdiv(span, 32) + 1,
+              kFewWhole, kFewLeast, most, p.grid_few, p.fill_few);
   if (p.rows)
-    plan_grid(T, B, Hkv, grp, 128, rows, cdiv(span, D == 256 ? 32 : 64) + 1, kRowsWhole, kRowsLeast, kRowsFill, p.grid_rows,
+    plan_grid(T, B, Hkv, grp, 128, rows, INT32_MAX, cdiv(span, D == 256 ? 32 : 64) + 1, kRowsWhole, kRowsLeast, kRowsFill, p.grid_rows,
               p.fill_rows);
   return p;
 }

@@ -257,6 +257,20 @@ def test_more_parts_than_places(dev, groups):
         assert float((got - want).norm() / want.norm()) <= 2 * (max(ctx) / 16) ** 0.5 * 2.0**-24
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_long_contexts_of_few_tokens_beside_prompts(dev, dtype, d):
+    """Contexts past 8192: requests of few rows are cut into parts in a launch of their own, whose blocks
+    their number bounds; rows of padding after them are either kernel's."""
+    s = Setup(dev, [300, 9001, 70, 12000], [150, 1, 70, 8], 4, 1, d, 64, dtype, seed=d)
+    s.check(s.attend())
+    s.check(s.attend(window=8500), window=8500)
+    for pad in (3, 200):
+        out = s.attend(torch.cat([s.q, torch.full((pad, 4, d), float("nan"), device=dev, dtype=dtype)]))
+        assert not out[len(s.q):].any()
+        s.check(out[: len(s.q)])
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_tensors_of_another_device_than_the_current_one(dev):
     """Calls run on their tensors' device, on its current stream, whatever the current device is; a tile
