@@ -434,7 +434,9 @@ int qs_plan_step(const int32_t* ring, int64_t ring_size, const int64_t* state, i
                  void* stream);
 
 /* Pages of requests with done[b] != 0, which hold lens[b] tokens, back to the ring's tail, in request
- * and column order; entries below 0 are passed over.  state_out = {head, new tail, 0}. */
+ * and column order; entries below 0 are passed over.  state_out = {head, new tail, 0}.  The ring has
+ * room for the pages that were taken from it, and is not checked for more: a page given back twice
+ * overwrites a free one's entry. */
 int qs_release_pages(int32_t* ring, int64_t ring_size, const int64_t* state, int64_t* state_out,
                      const int32_t* tables, int64_t ld_table, int64_t width, const int32_t* lens,
                      const uint8_t* done, int64_t B, int64_t page_size, void* stream);
@@ -467,7 +469,8 @@ int qs_kv4_read(const uint8_t* cache, int64_t pages, int64_t page_size, int Hkv,
                 const int64_t* slots, int64_t n, void* k_out, void* v_out, int out_dtype,
                 void* stream);
 
-/* Workspace bytes of qs_kv4_attend for these sizes (0: none).  The workspace's first 32 KiB are zero
+/* Workspace bytes of qs_kv4_attend for these sizes (0: none; 34 MB at most with heads of 128, 68 with
+ * 256: the parts of as many blocks as run at once).  The workspace's first 32 KiB are zero
  * before its first use, and every call leaves them zero: calls that follow one another on a stream
  * can share one of the largest size, calls that overlap need workspaces of their own. */
 size_t qs_kv4_attend_workspace_bytes(int64_t T, int64_t B, int Hkv, int Hq, int D, int64_t page_size,

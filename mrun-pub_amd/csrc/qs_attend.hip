@@ -11,15 +11,15 @@
 // running maximum, one pass over the cache.  Blocks share the requests' tokens out among themselves
 // (pick_part); where several take parts of one tile's tokens, the last of them to finish joins them.
 //
-// Measured on an MI355X whose copy reaches 5.1 TB/s and whose 8192^3 bf16 product 1155 TFLOP/s (in
-// brackets other cards, not rated), heads of 128, a call from Python:
-//   1 token over 513, 12 + 2 heads           7.3 us  latency: plan, pages, first codes, 3 steps, join
-//   29 requests up to 8100, 32 + 8 heads    31.5 us  3.5 TB/s; the vector unit unpacks 60% of it
-//   2 contexts of 131000, fp16              68.7 us  4.4 TB/s (65)
-//   11 requests of 5 tokens up to 6001      18.4 us  latency
-//   4095 tokens, 32 + 8 heads                188 us  731 TFLOP/s (171, 801): vector operations 49% and
-//                                                    products 38% of the cycles, hardly at once
-//   chunks of 701, window 1024, fp32 of 64  36.1 us  153 TFLOP/s, the fp32 product's own rate
+// Measured on an MI355X whose copy reaches 4.84 TB/s and whose 8192^3 bf16 product 1217 TFLOP/s, heads
+// of 128, a call from Python:
+//   1 token over 513, 12 + 2 heads           7.4 us  latency: plan, pages, first codes, 3 steps, join
+//   29 requests up to 8100, 32 + 8 heads    30.8 us  3.6 TB/s; the vector unit unpacks 58% of it
+//   2 contexts of 131000, fp16              65.4 us  4.6 TB/s
+//   11 requests of 5 tokens up to 6001      18.6 us  latency
+//   4095 tokens, 32 + 8 heads                171 us  803 TFLOP/s: vector operations 49% and products 38%
+//                                                    of the cycles, hardly at once
+//   chunks of 701, window 1024, fp32 of 64  36.3 us  152 TFLOP/s, the fp32 product's own rate
 #include <atomic>
 #include <type_traits>
 
@@ -61,7 +61,8 @@ struct AttendArgs {
 //
 // bf16 activations multiply fp16: cache values are code * s + lo in fp16 (one rounding, 2^-11),
 // queries are exact, since a row of bf16 is first divided by a power of two that takes its largest
-// value below 1 (8 bits fit fp16's 11 down to 2^-17 of that), weights are fp16.
+// value below 1 (8 bits fit fp16's 11 down to 2^-17 of that; smaller values keep steps of 2^-24 of the
+// row's largest), weights are fp16.
 //
 // fp16 and fp32 activations, whose own rounding is no coarser than that, multiply the codes, which
 // both 16-bit types hold exactly: q.k = s (q.code) + lo sum(q) a group, and for the output the
@@ -561,6 +562,11 @@ __device__ __forceinline__ bool last_part(const AttendArgs& a, const Work& w, in
 // where few waves run.  kLean: room for up to twice the waves where their number does that, in blocks
 // of half the size, which share out ragged requests more evenly.  kDeep: the same in blocks of eight
 // waves, which leave half the parts to join where long contexts of few requests are cut into dozens.
+// Single tokens of ragged requests, 32 + 8 heads of 128, us of kAhead / kLean / kDeep:
+//   few steps    bf16 1 of 32768 17.4 / 20.9 / 19.7, 16 up to 2048 13.1 / 15.7 / 16.6; fp16 1 of 32768 18.7 / 21.3
+//   few tiles    bf16 2 up to 131072 50.8 / 54.5 / 50.6, 8 up to 16384 24.4 / 25.7 / 24.3; fp16 47.1 / 51.1, 28.4 / 28.4
+//   neither      bf16 16 up to 8192 28.1 / 27.5 / 26.5, 64 up to 2000 36.0 / 27.5 / 25.8; fp16 46.9 / 28.7, 39.5 / 30.6
+//   short tiles  bf16 40 up to 250 10.5 / 7.8, 64 up to 64 12.1 / 7.4, 60 of 5 tokens up to 34 18.1 / 10.4
 enum { kAhead, kLean, kDeep };
 constexpr bool few_wide(int kind, int D, int rt) { return D * rt >= (kind == 2 ? 256 : 512); }
 constexpr int few_waves(int kind, int D, int rt, int form) {  // a SIMD, as the registers allow
@@ -582,7 +588,11 @@ constexpr bool few_used(int kind, int D, int rt, int form) {
 }
 // Whether registers hold two tiles of 16 rows.
 constexpr bool few_pairs(int kind, int D) { return kind == 0 || D < 256; }
-constexpr int kFewLeast = 16, kFewWhole = 32;    // steps of a part at least, steps that stay whole
+// Steps of a part at least, and steps that stay whole.  32 + 8 heads, us with parts and without: a token
+// over 4000 12.1 and 24.6, over 2000 12.1 and 15.2, over 1000 11.3 and 10.3 (parts of 8 from 16 on: 11.7,
+// 10.9 and 10.7, but 10.6 where 8.0 over 600, and 13.1 where 11.8 for 16 over 1000); 200 rows of tokens
+// over 4000 39 and 98, over 1000 19.4 and 29.8 (parts of 2 from 4 on: 39.9 and 21.8, of 8 from 16 on: 39.1 and 30.8).
+constexpr int kFewLeast = 16, kFewWhole = 32;
 constexpr int kRowsLeast = 4, kRowsWhole = 8, kRowsFill = 512;
 
 template <class T, int D, int RT, int FORM>

@@ -26,7 +26,8 @@ def free_pages(pages: int, device, *, first: int = 0) -> tuple[torch.Tensor, tor
 
 
 class StepPlan(NamedTuple):
-    """One step's metadata; every tensor is on the device.
+    """One step's metadata; every tensor is on the device, all six in one allocation, which the last of
+    them that is held keeps.
 
     ``slots [tokens] int64`` (page * page_size + offset; -1 for a row of padding or one whose page
     was missing), ``positions [tokens] int32``, ``requests [tokens] int32`` (-1 for padding),
@@ -86,7 +87,8 @@ def release_pages(
 ) -> torch.Tensor:
     """The pool's new state after the pages of requests with ``done[b]`` (bool), which hold
     ``lens[b]`` tokens, went back to the ring, in request order.  Table entries of -1 are passed
-    over; the tables keep their entries."""
+    over; the tables keep their entries.  The ring has room for the pages that were taken from it and
+    is not checked for more: a page given back twice overwrites a free one's entry."""
     _pool(ring, free_state)
     B = int(lens.numel())
     held = _lengths("lens", lens, B)
