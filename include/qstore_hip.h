@@ -482,7 +482,7 @@ size_t qs_kv4_attend_workspace_bytes(int64_t T, int64_t B, int Hkv, int Hq, int 
  * tokens of a column past width, or whose entry is not in [0, pages), are not seen; a query that sees
  * nothing, or a row after the last request's, gives zeros.  max_query / max_context bound the
  * requests (0 or larger than the truth is fine; they only choose the split).  starts does not
- * decrease.  out [T, Hq, D] contiguous.  q heads are 16-byte aligned. */
+ * decrease: where it does, any rows may be left unwritten.  out [T, Hq, D] contiguous.  q heads are 16-byte aligned. */
 int qs_kv4_attend(const void* q, int dtype, int64_t ldq_t, int64_t ldq_h, const uint8_t* cache,
                   int64_t pages, int64_t page_size, int Hkv, int Hq, int D, const int32_t* tables,
                   int64_t ld_table, int64_t width, const int32_t* starts, const int32_t* context,

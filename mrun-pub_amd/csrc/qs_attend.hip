@@ -319,9 +319,12 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
   const int b0 = me * each < a.B + 1 ? me * each : a.B + 1, b1 = b0 + each < a.B + 1 ? b0 + each : a.B + 1;
   int64_t q0 = 0;
   int n = 0, ctx = 0, tiles = 0, steps = 0;
+  bool falls = false;
   auto look = [&](int b) {
     q0 = start_of(a, b);
-    n = new_of(a, b, q0);
+    const int64_t q1 = b < a.B ? start_of(a, b + 1) : a.T;
+    falls |= q1 < q0;
+    n = q1 > q0 ? (int)(q1 - q0) : 0;
     const int rows = n * a.grp;
     tiles = mine(a, rows) ? (rows + R - 1) / R : 0;
     ctx = context_of(a, b);
@@ -350,7 +353,12 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
     sum += (float)tiles * (float)steps;
   }
   const float most = (float)a.blocks / (float)a.Hkv;
-  const float total = total_of(sum);
+  const float total = total_of(falls ? __builtin_inff() : sum);
+  if (total == __builtin_inff()) {  // starts that decrease: requests would share rows, and no bound here would hold
+    Work t;
+    t.any = false;
+    return t;
+  }
   float size = total * 1.00001f / most + 1.f;  // sums of rounded products: never too small
   if (size < (float)a.least) size = (float)a.least;
   int count, before, place;

@@ -271,6 +271,19 @@ def test_long_contexts_of_few_tokens_beside_prompts(dev, dtype, d):
         s.check(out[: len(s.q)])
 
 
+@pytest.mark.parametrize("B,new,ctx", [(6, 1, 5000), (6, 60, 5000), (70, 1, 3000), (70, 40, 3000)])
+def test_starts_that_decrease_leave_later_calls_alone(dev, B, new, ctx):
+    """Such starts are a caller's mistake that only the GPU sees.  Nothing is read or written out of
+    place for them, and what calls share, the counters of finished parts, is as it was."""
+    s = Setup(dev, [ctx] + [200] * (B - 1), [new] * B, 4, 1, 64, 16, torch.bfloat16, seed=B)
+    want = s.attend()
+    starts = s.starts.copy()
+    starts[1:-1:2] = starts[-1]  # every other request has all rows, the next ones none
+    out = torch.zeros_like(s.q)
+    kv4.attend(s.q, s.cache, 0, s.tables, i32(starts, dev), i32(s.ctx, dev), max_query=new, max_context=ctx, out=out)
+    assert torch.equal(s.attend(), want)
+
+
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_tensors_of_another_device_than_the_current_one(dev):
     """Calls run on their tensors' device, on its current stream, whatever the current device is; a tile
