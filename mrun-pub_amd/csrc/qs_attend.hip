@@ -382,8 +382,8 @@ __device__ __forceinline__ Work pick_part(const AttendArgs& a, int y, float* s_s
       }
       round = 3;
     }
-    // Blocks and places before this thread's, in one sum: both are below 2^15, the tiles' bound of
-    // 4 a.blocks (plan_grid) and a block more for each part.
+    // Blocks and places before this thread's, in one sum: both are below 2^15, at most 4096 tiles
+    // (plan_grid) and a block more for each of 1024 parts, while starts do not decrease.
     const int both = count | cut << 16;
     int sum = wave_scan(both), all = __builtin_amdgcn_readlane(sum, 63);
     sum -= both;
